@@ -15,7 +15,7 @@
  *     on `stream`: lsdm_sample_steps_invariant also runs the dense encoder chains of alternate steps on a side stream of the context
  *     (forked from `stream` by an event and joined back before the call's last launches; LSDM_STREAMS=1 keeps one stream) -- work the
  *     caller enqueues on `stream` after the call sees all of its results.
- *   - one context per (process, device); a context is not thread-safe; different contexts are independent.
+ *   - one context per (process, device) (the operators at the end take none); a context is not thread-safe; different contexts are independent.
  *   - all floating-point tensors are fp32, dense, row-major; timesteps / FPS starts are int64 (torch.long),
  *     internal index outputs are int32.
  *   - fixed by the model (model/sdm.py:19-22, pointnet2.py:46-55): 9 object slots, 1024 points per cloud, latent 128.
@@ -219,6 +219,64 @@ LSDM_API int lsdm_train_step(lsdm_train* s, int B, int flags, const float* x_sta
  * max-pool routes the gradient.  (Two neighbours whose activations differ in the last bits make that choice depend on the summation
  * order of the layer before; the parity test injects these choices into the oracle and checks that every difference IS such a near-tie.) */
 LSDM_API int lsdm_train_read(lsdm_train* s, const char* name, void* host_dst, int64_t capacity_bytes, int64_t* nbytes);
+
+/* ---- operators of the text towers (model/sdm.py:146-149, 245-285): dense layer, layer norm, 8-bit activation checkpoints ---------------
+ * The reference runs its CLIP / BERT tower on the packages' eager layers; these are the layers of such a tower's residual blocks, forward and
+ * backward.  They take no context and keep nothing between calls: any thread, `device` and `stream`; every buffer is the caller's (scratch
+ * memory included: *_workspace says how much, 16-byte aligned, free to be reused once the call's work on `stream` is done).  A failing call's
+ * message is lsdm_last_error(NULL) of the same thread.  Sums, statistics and activations are evaluated in fp32 whatever the type; results are
+ * rounded once.  Results do not depend on the schedule (no atomics).  Buffers must not overlap unless said otherwise. */
+typedef enum { LSDM_F32 = 0, LSDM_BF16 = 1, LSDM_F16 = 2 } lsdm_dtype;
+typedef enum {
+    LSDM_ACT_NONE = 0,
+    LSDM_ACT_RELU,          /* max(z, 0)                                                   */
+    LSDM_ACT_GELU,          /* z Phi(z), Phi the normal distribution function (BERT)       */
+    LSDM_ACT_QUICK_GELU,    /* z s(1.702 z), s(t) = 1 / (1 + exp(-t)) (CLIP)               */
+    LSDM_ACT_SILU,          /* z s(z)                                                      */
+    LSDM_ACT_SIGMOID,       /* s(z)                                                        */
+    LSDM_ACT_TANH,          /* tanh z (BERT's pooler)                                      */
+    LSDM_ACT_COUNT
+} lsdm_activation;
+enum {
+    LSDM_OP_PARAM_F32 = 1,  /* bias / norm weight and bias (and their gradients) are fp32; otherwise of the call's dtype */
+    LSDM_OP_DERIV8 = 2,     /* `deriv` holds 8-bit codes u = rint(192 a'(z)) + 32 (255: NaN) instead of the call's dtype */
+    /* lsdm_linear_workspace only: what the call will do and which rows are not made of whole, aligned 16-byte pieces */
+    LSDM_OP_BACKWARD = 4, LSDM_OP_DX = 8, LSDM_OP_DW = 16, LSDM_OP_DB = 32, LSDM_OP_DERIV = 64, LSDM_OP_CODES = 128,
+    LSDM_OP_X_UNALIGNED = 256, LSDM_OP_W_UNALIGNED = 512, LSDM_OP_DY_UNALIGNED = 1024
+};
+
+/* y = a(x w^T + bias) + residual.  x (M,K) with row stride ldx, w (N,K) with row stride ldw, bias (N) or NULL, residual (M,N) with row stride
+ * ldr or NULL (it may be y itself), y (M,N) dense.  deriv: NULL, or (M,N) that receives a'(z) for lsdm_linear_backward (untouched without an
+ * activation).  1 <= M, N, K <= 2^30. */
+LSDM_API int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
+                int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, void* deriv, void* ws, int64_t ws_bytes, void* stream);
+/* dz = dy a'(z);  dx = dz w,  dw = dz^T x,  db = column sums of dz (each NULL: not wanted; the residual's gradient is dy).  dy (M,N) with row
+ * stride lddy; deriv as lsdm_linear wrote it, NULL without an activation; x as in the forward call, or its 8-bit checkpoint codes / exps
+ * (lsdm_pack8) with x NULL; dx (M,K), dw (N,K), db (N) dense.  dz is rounded to the call's dtype in front of the two products (they run on the
+ * matrix cores of that type); db sums the unrounded values. */
+LSDM_API int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N, int64_t K, const void* dy, int64_t lddy, const void* deriv,
+                const void* x, int64_t ldx, const void* codes, const void* exps, const void* w, int64_t ldw, void* dx, void* dw, void* db, void* ws,
+                int64_t ws_bytes, void* stream);
+/* bytes of scratch memory of either call (flags: the enum above), or a negative lsdm_status */
+LSDM_API int64_t lsdm_linear_workspace(int dtype, int flags, int64_t M, int64_t N, int64_t K);
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over the last axis, var = mean (x - mean)^2.  x (rows,D) with row stride ldx, y (rows,D) dense, w and b
+ * (D) or NULL (1 and 0), 1 <= D <= 16384.  For the backward pass: mean, rstd (rows) fp32 or NULL; codes (rows,D) int8 with exps
+ * (rows,ceil(D/32)) uint8, the 8-bit checkpoint of the normalised rows h, or both NULL. */
+LSDM_API int lsdm_layer_norm(int device, int dtype, int flags, int64_t rows, int64_t D, const void* x, int64_t ldx, const void* w, const void* b, float eps,
+                void* y, float* mean, float* rstd, void* codes, void* exps, void* stream);
+/* g = dy w;  dx = rstd (g - mean g - h mean(g h)),  dw = sum over rows of dy h,  db = sum of dy (each NULL: not wanted).  h comes from x, mean and
+ * rstd, or from codes / exps (x and mean are not read then).  ws: lsdm_layer_norm_workspace bytes where dw or db is wanted. */
+LSDM_API int lsdm_layer_norm_backward(int device, int dtype, int flags, int64_t rows, int64_t D, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                const void* codes, const void* exps, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db, void* ws,
+                int64_t ws_bytes, void* stream);
+LSDM_API int64_t lsdm_layer_norm_workspace(int64_t rows, int64_t D);
+
+/* 8-bit checkpoint of x (rows,D), row stride ldx: groups of 32 consecutive values of a row share the step 2^e, e = max(floor(log2 max|x|) - 6,
+ * -126): codes (rows,D) int8 = x / 2^e rounded to nearest even, clamped to +-127; exps (rows,ceil(D/32)) uint8 = e + 127, or 255 for a group that
+ * holds an infinity or a NaN.  lsdm_unpack8 writes the values codes 2^e (exact in every dtype; NaN where exps is 255) to out (rows,D) dense. */
+LSDM_API int lsdm_pack8(int device, int dtype, int64_t rows, int64_t D, const void* x, int64_t ldx, void* codes, void* exps, void* stream);
+LSDM_API int lsdm_unpack8(int device, int dtype, int64_t rows, int64_t D, const void* codes, const void* exps, void* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,7 +19,7 @@ class LsdmError(RuntimeError):
 
 _lib = None
 
-_vp, _i, _f, _d = C.c_void_p, C.c_int, C.c_float, C.c_double
+_vp, _i, _f, _d, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_int64
 _SIGNATURES = {
     "lsdm_create": (_i, [C.POINTER(_vp), _i]),
     "lsdm_destroy": (_i, [_vp]),
@@ -51,6 +51,14 @@ _SIGNATURES = {
     "lsdm_train_bind": (_i, [_vp, C.c_char_p, _vp, _vp, C.c_int64]),
     "lsdm_train_read": (_i, [_vp, C.c_char_p, _vp, C.c_int64, C.POINTER(C.c_int64)]),
     "lsdm_train_step": (_i, [_vp, _i, _i] + [_vp] * 12 + [_f, _f] + [_vp] * 4),
+    "lsdm_linear": (_i, [_i] * 4 + [_i64] * 3 + [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "lsdm_linear_backward": (_i, [_i] * 3 + [_i64] * 3 + [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "lsdm_linear_workspace": (_i64, [_i] * 2 + [_i64] * 3),
+    "lsdm_layer_norm": (_i, [_i] * 3 + [_i64] * 2 + [_vp, _i64, _vp, _vp, _f] + [_vp] * 6),
+    "lsdm_layer_norm_backward": (_i, [_i] * 3 + [_i64] * 2 + [_vp, _i64, _vp, _i64] + [_vp] * 9 + [_i64, _vp]),
+    "lsdm_layer_norm_workspace": (_i64, [_i64] * 2),
+    "lsdm_pack8": (_i, [_i] * 2 + [_i64] * 2 + [_vp, _i64] + [_vp] * 3),
+    "lsdm_unpack8": (_i, [_i] * 2 + [_i64] * 2 + [_vp] * 4),
 }
 EXPORTS = tuple(_SIGNATURES)
 

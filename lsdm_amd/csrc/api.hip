@@ -1135,6 +1135,8 @@ int check_ready(lsdm_ctx* c, int B, bool need_sched) {
 
 }  // namespace
 
+void lsdm::set_thread_error(const char* msg) { g_create_error = msg; }
+
 extern "C" {
 
 int lsdm_create(lsdm_ctx** out, int device) {

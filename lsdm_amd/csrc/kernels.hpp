@@ -198,4 +198,7 @@ void launch_denoise_r(int np, const DenseH& blob, const Lin& pwt, const StepCoef
                       float* out_sample, int num_cus, hipStream_t st, long long pcd_step = 0, long long o12_step = 0);
 // (pcd_step / o12_step != 0: step s of the launch reads pcd + s * pcd_step, o12 + s * o12_step -- the steps of a loop-invariant group)
 
+// api.hip: the message lsdm_last_error(NULL) returns on this thread
+void set_thread_error(const char* msg);
+
 }  // namespace lsdm

@@ -1,0 +1,156 @@
+// Shared pieces of the public operators (ops_gemm.hip, ops_norm.hip, ops_pack8.hip, ops_api.hip): element types, 8-element row pieces, the
+// activations with their derivatives, the 8-bit checkpoint format, and the launchers the C entry points call.
+#pragma once
+#include "common.hpp"
+
+namespace lsdm {
+namespace ops {
+
+typedef __bf16 bfrag __attribute__((ext_vector_type(8)));
+typedef _Float16 hfrag __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+enum OpAct { OP_NONE = 0, OP_RELU, OP_GELU, OP_QUICK_GELU, OP_SILU, OP_SIGMOID, OP_TANH, OP_ACT_COUNT };
+
+template <class T> struct Half8;                                   // 8 elements of a 16-bit type as one 16-byte piece
+template <> struct Half8<__bf16> { typedef bfrag type; };
+template <> struct Half8<_Float16> { typedef hfrag type; };
+
+// ---- eight consecutive elements of a row <-> fp32 (the row piece is 16-byte aligned, 32 bytes long in fp32) ----
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    const typename Half8<T>::type r = *reinterpret_cast<const typename Half8<T>::type*>(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    typename Half8<T>::type r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
+    *reinterpret_cast<typename Half8<T>::type*>(p) = r;
+}
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
+    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+// the same for a piece that may be unaligned or cut short: n valid elements (the others read as 0 / are not written)
+template <class T>
+__device__ __forceinline__ void load8n(const T* p, int n, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
+}
+template <class T>
+__device__ __forceinline__ void store8n(T* p, int n, const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) p[j] = (T)v[j];
+}
+// a parameter vector (bias, norm weight) is of the operand's type or fp32
+template <class T>
+__device__ __forceinline__ float param(const void* p, int is_f32, long long i) {
+    return is_f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
+}
+template <class T>
+__device__ __forceinline__ void store_param(void* p, int is_f32, long long i, float v) {
+    if (is_f32) static_cast<float*>(p)[i] = v; else static_cast<T*>(p)[i] = (T)v;
+}
+
+// ---- activations: y = a(z) and, where asked for, d = a'(z) ----
+// fp32 results use the libm functions; 16-bit results the hardware exp2 / reciprocal forms of common.hpp (absolute error <= 3e-7, four orders
+// below a bf16 step of a value near one).  NaN stays NaN in y for every activation; relu'(NaN) = 0 (the comparison z > 0).
+template <class T>
+__device__ __forceinline__ void act_eval(int act, float z, bool want, float& y, float& d) {
+    constexpr bool fast = sizeof(T) == 2;
+    d = 1.0f;
+    switch (act) {
+        case OP_RELU: y = z <= 0.0f ? 0.0f : z; d = z > 0.0f ? 1.0f : 0.0f; break;
+        case OP_GELU: {
+            const float x = fabsf(z) * 0.70710678118654752440f;
+            if constexpr (fast) {
+                const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f)), ex = __expf(-x * x);
+                float pl = fmaf(t, 1.061405429f, -1.453152027f);
+                pl = fmaf(t, pl, 1.421413741f);
+                pl = fmaf(t, pl, -0.284496736f);
+                pl = fmaf(t, pl, 0.254829592f);
+                const float q = 0.5f * (pl * t) * ex, phi = z < 0.0f ? q : 1.0f - q;
+                y = z * phi;
+                d = fmaf(z * 0.39894228040143267794f, ex, phi);
+            } else {
+                const float phi = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+                y = z * phi;
+                if (want) d = phi + z * 0.39894228040143267794f * expf(-0.5f * z * z);
+            }
+            break;
+        }
+        case OP_QUICK_GELU:
+        case OP_SILU: {
+            const float c = act == OP_SILU ? 1.0f : 1.702f;
+            const float s = fast ? sigmoid_fast(c * z) : sigmoidf(c * z);
+            y = z * s;
+            d = s * fmaf(c * z, 1.0f - s, 1.0f);
+            break;
+        }
+        case OP_SIGMOID: y = fast ? sigmoid_fast(z) : sigmoidf(z); d = y * (1.0f - y); break;
+        case OP_TANH: y = tanhf(z); d = fmaf(-y, y, 1.0f); break;
+        default: y = z; break;
+    }
+}
+
+// a'(z) in 8 bits: u = rint(192 a') + 32.  Every derivative above lies in [-0.13, 1.13], i.e. codes 7 .. 249; 0 and 1 (relu) are exact; the
+// error is at most 1/384.  Code 255 stands for NaN.
+__device__ __forceinline__ unsigned deriv_code(float d) {
+    const float u = fminf(fmaxf(rintf(192.0f * d) + 32.0f, 0.0f), 254.0f);
+    return d != d ? 255u : (unsigned)u;
+}
+__device__ __forceinline__ float deriv_value(unsigned u) {
+    return u == 255u ? __builtin_nanf("") : (float)((int)u - 32) * (1.0f / 192.0f);
+}
+
+// ---- 8-bit checkpoint: groups of kGroup8 consecutive values of a row share a power-of-two step 2^e ----
+// m = max |x| of the group, e = max(floor(log2 m) - 6, -126), q = clamp(rint(x 2^-e), +-127); stored: q (int8), e + 127 (uint8), 255 for a
+// group that holds an infinity or a NaN (it decodes to NaN: a checkpoint never hides an overflow).  q 2^e has at most 7 significant bits, so it
+// is exact in fp32, bf16 and fp16.
+constexpr int kGroup8 = 32;
+constexpr unsigned kNanExp8 = 255u;
+__device__ __forceinline__ unsigned exp8_of_amax(float m) {        // m >= 0, NaN or inf for a non-finite group
+    const int E = (int)(__builtin_bit_cast(unsigned, m) >> 23);     // biased exponent (0: zero or subnormal)
+    return E == 255 ? kNanExp8 : (unsigned)(E - 6 > 1 ? E - 6 : 1);
+}
+__device__ __forceinline__ float exp8_step(unsigned b) { return b == kNanExp8 ? __builtin_nanf("") : __builtin_bit_cast(float, b << 23); }
+// 2^-e: e + 127 in [1, 248] -> the reciprocal's biased exponent 254 - b is in [6, 253]; b = 255 gives 0 (codes of such a group are 0)
+__device__ __forceinline__ float exp8_inv(unsigned b) { return b == kNanExp8 ? 0.0f : __builtin_bit_cast(float, (254u - b) << 23); }
+__device__ __forceinline__ int code8(float x, float inv) {
+    const float v = rintf(x * inv);
+    return (int)fminf(fmaxf(v, -127.0f), 127.0f);                   // (non-finite groups: inv = 0, the NaN of inf * 0 is dropped by fmaxf)
+}
+
+// ---- kernels' argument blocks and launchers ----
+struct Epilogue {
+    const void* bias = nullptr; int bias_f32 = 0;
+    const void* res = nullptr; long long ldr = 0;
+    void* out = nullptr; long long ldo = 0;
+    void* deriv = nullptr; long long ldd = 0; int deriv8 = 0;      // a'(z) for the backward pass, in the operand's type or as a code byte
+    int act = OP_NONE;
+    int vec = 0;                                                    // every row piece of 8 outputs is whole and 16-byte aligned
+};
+struct GemmArgs {
+    const void *A = nullptr, *B = nullptr;                          // C(m, n) = sum_k A(m, k) B(n, k)
+    long long lda = 0, ldb = 0;                                     // row strides in elements
+    int M = 0, N = 0, K = 0;
+    int tiles_m = 0, tiles_n = 0, splits = 1, kchunk = 0;
+    float* part = nullptr;                                          // splits > 1: (splits, M, N) partial sums
+    Epilogue e;
+};
+
+enum Layout { KK = 0, KM = 1, MM = 2 };                             // contraction axis contiguous in (A and B), (A only), (neither)
+
+}  // namespace ops
+}  // namespace lsdm

@@ -1,0 +1,351 @@
+// C entry points of the public operators (include/lsdm_hip.h: lsdm_linear*, lsdm_layer_norm*, lsdm_pack8, lsdm_unpack8): argument checks, the
+// choice of a kernel variant, and the layout of the caller's scratch memory.  They need no context: any thread, any device, any stream; a
+// failure's message is the calling thread's (lsdm_last_error(NULL)).
+#include "../../include/lsdm_hip.h"
+
+#include <cstdarg>
+#include <cstdio>
+
+#include "kernels.hpp"
+#include "ops_launch.hpp"
+
+using namespace lsdm;
+using namespace lsdm::ops;
+
+namespace {
+
+int refuse(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_thread_error(buf);
+    return code;
+}
+
+struct OnDevice {                                 // the entry point's device, the caller's restored on return
+    int prev = -1;
+    bool ok = false;
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev == device) { ok = true; prev = -1; return; }
+        ok = device >= 0 && hipSetDevice(device) == hipSuccess;
+        if (!ok) { (void)hipGetLastError(); refuse(LSDM_ERR_HIP, "hipSetDevice(%d) failed", device); }
+    }
+    ~OnDevice() { if (prev >= 0) (void)hipSetDevice(prev); }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? LSDM_OK : refuse(LSDM_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+constexpr int64_t kMaxSize = (int64_t)1 << 30;
+constexpr int kCUs = 256;                         // MI355X
+int esize(int dtype) { return dtype == LSDM_F32 ? 4 : 2; }
+bool dtype_ok(int d) { return d == LSDM_F32 || d == LSDM_BF16 || d == LSDM_F16; }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// rows of `width` elements `ld` apart whose 16-byte pieces are whole and aligned
+bool rows16(const void* p, int64_t ld, int64_t width, int es) { return aligned16(p) && ld * es % 16 == 0 && width * es % 16 == 0; }
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// carves the caller's scratch memory; with base == NULL it only adds up
+struct Carve {
+    char* base;
+    int64_t used = 0;
+    void* take(int64_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += up(bytes, 256);
+        return p;
+    }
+};
+
+// Tile and split of C (M, N) with contraction K.  A launch costs its rounds of work-groups (256 CUs x resident work-groups) times the steps a
+// work-group walks; the estimate below is that product with the measured time of a step, plus the join of a split contraction (its partial
+// sums are written and read once).
+GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
+    struct Kind { int tile, resident; float step, fixed; };        // us per 128-byte step with `resident` work-groups on a CU; prologue + epilogue
+    static const Kind half[] = {{256, 1, 1.05f, 6.0f}, {128, 2, 0.60f, 4.5f}, {64, 3, 0.45f, 3.5f}};
+    static const Kind single[] = {{128, 2, 3.6f, 6.0f}, {64, 3, 1.6f, 4.0f}};
+    const int bk = 128 / esize(dtype);
+    const int64_t steps = (K + bk - 1) / bk;
+    GemmPlan best;
+    float best_us = 0.0f;
+    const Kind* kinds = dtype == LSDM_F32 ? single : half;
+    const int nk = dtype == LSDM_F32 ? 2 : 3;
+    for (int i = 0; i < nk; ++i) {
+        const Kind& k = kinds[i];
+        const int64_t tm = (M + k.tile - 1) / k.tile, tn = (N + k.tile - 1) / k.tile, tiles = tm * tn;
+        for (int s = 1; s <= 32; s = s < 4 ? s + 1 : s * 2) {
+            if (s > 1 && steps < 2 * s) break;
+            const int64_t per = (steps + s - 1) / s, used = steps ? (steps + per - 1) / per : 1;
+            if (used != s) continue;
+            const int64_t rounds = (tiles * s + kCUs * k.resident - 1) / (kCUs * k.resident);
+            float us = (float)rounds * ((float)per * k.step + k.fixed);
+            if (s > 1) us += 4.0f + (float)(s + 1) * (float)M * (float)N * 4.0f / 3.0e6f;
+            if (best.tile == 0 || us < best_us) {
+                best_us = us;
+                best.tile = k.tile; best.tiles_m = (int)tm; best.tiles_n = (int)tn; best.splits = s; best.kchunk = (int)(per * bk);
+            }
+        }
+    }
+    return best;
+}
+
+int64_t part_bytes(const GemmPlan& p, int64_t M, int64_t N) { return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0; }
+
+// work-groups of a preparation pass: about 2048 in all, at least eight rows each
+int prep_chunks(int64_t rows, int64_t cols) {
+    const int64_t cb = (cols + 255) / 256;
+    int64_t c = 2048 / cb;
+    if (c > (rows + 7) / 8) c = (rows + 7) / 8;
+    if (c > 1024) c = 1024;
+    return c < 1 ? 1 : (int)c;
+}
+
+constexpr int64_t kFewRows = 64;                  // products with at most this many rows run on rows_kernel
+
+struct Fwd { bool rows, xpad, wpad; GemmPlan p; void *x, *w; float* part; int64_t bytes; };
+Fwd forward_layout(int dtype, int64_t M, int64_t N, int64_t K, bool x_ok, bool w_ok, void* ws) {
+    Fwd f{};
+    Carve c{static_cast<char*>(ws)};
+    f.rows = M <= kFewRows;
+    if (!f.rows) {
+        const int64_t kp = up(K, 8);
+        f.xpad = !x_ok; f.wpad = !w_ok;
+        f.p = plan(M, N, K, dtype);
+        if (f.xpad) f.x = c.take(M * kp * esize(dtype));
+        if (f.wpad) f.w = c.take(N * kp * esize(dtype));
+        f.part = static_cast<float*>(c.take(part_bytes(f.p, M, N)));
+    }
+    f.bytes = c.used;
+    return f;
+}
+
+struct Bwd { bool dz, xpad, wpad; int chunks; int64_t ldz, kp; GemmPlan px, pw; void *z, *x, *w; float *cs, *partx, *partw; int64_t bytes; };
+Bwd backward_layout(int dtype, int64_t M, int64_t N, int64_t K, bool dx, bool dw, bool db, bool deriv, bool codes, bool dy_ok, bool x_ok, bool w_ok,
+                    void* ws) {
+    Bwd b{};
+    Carve c{static_cast<char*>(ws)};
+    const int es = esize(dtype);
+    b.kp = up(K, 8); b.ldz = up(N, 8);
+    b.dz = (dx || dw) && (deriv || !dy_ok);
+    b.xpad = dw && (codes || !x_ok);
+    b.wpad = dx && !w_ok;
+    b.chunks = prep_chunks(M, b.ldz);
+    if (b.dz) b.z = c.take(M * b.ldz * es);
+    if (db) b.cs = static_cast<float*>(c.take((int64_t)b.chunks * N * 4));
+    if (b.xpad) b.x = c.take(M * b.kp * es);
+    if (b.wpad) b.w = c.take(N * b.kp * es);
+    if (dx) { b.px = plan(M, K, N, dtype); b.partx = static_cast<float*>(c.take(part_bytes(b.px, M, K))); }
+    if (dw) { b.pw = plan(N, K, M, dtype); b.partw = static_cast<float*>(c.take(part_bytes(b.pw, N, K))); }
+    b.bytes = c.used;
+    return b;
+}
+
+void copy_padded(int dtype, const void* src, int64_t lds, int64_t rows, int64_t n, void* dst, int64_t ldd, hipStream_t st) {
+    PrepArgs a;
+    a.src = src; a.lds = lds; a.dst = dst; a.ldd = ldd; a.rows = rows; a.n = (int)n;
+    a.vec_src = rows16(src, lds, 8, esize(dtype));
+    launch_prep(dtype, a, prep_chunks(rows, ldd), st);
+}
+
+int check_linear(int dtype, int64_t M, int64_t N, int64_t K) {
+    if (!dtype_ok(dtype)) return refuse(LSDM_ERR_ARG, "lsdm_linear: unknown dtype %d", dtype);
+    if (M < 1 || N < 1 || K < 1 || M > kMaxSize || N > kMaxSize || K > kMaxSize)
+        return refuse(LSDM_ERR_ARG, "lsdm_linear: sizes (%lld, %lld, %lld) must lie in [1, 2^30]", (long long)M, (long long)N, (long long)K);
+    return LSDM_OK;
+}
+
+int norm_grid(int64_t rows, int D, bool vec, bool backward) {
+    const int rpg = norm_rows_per_group(D, vec);
+    const int64_t need = (rows + rpg - 1) / rpg;
+    // every work-group loads the parameters once; the backward pass also leaves one partial row each: as many as are resident, no more
+    const int64_t cap = backward ? 2 * kCUs : 8 * kCUs;
+    return (int)(need < cap ? need : cap);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t lsdm_linear_workspace(int dtype, int flags, int64_t M, int64_t N, int64_t K) {
+    if (check_linear(dtype, M, N, K) != LSDM_OK) return LSDM_ERR_ARG;
+    const bool x_ok = !(flags & LSDM_OP_X_UNALIGNED), w_ok = !(flags & LSDM_OP_W_UNALIGNED);
+    if (!(flags & LSDM_OP_BACKWARD)) return forward_layout(dtype, M, N, K, x_ok, w_ok, nullptr).bytes;
+    return backward_layout(dtype, M, N, K, flags & LSDM_OP_DX, flags & LSDM_OP_DW, flags & LSDM_OP_DB, flags & LSDM_OP_DERIV, flags & LSDM_OP_CODES,
+                           !(flags & LSDM_OP_DY_UNALIGNED), x_ok, w_ok, nullptr).bytes;
+}
+
+int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                const void* bias, const void* residual, int64_t ldr, void* y, void* deriv, void* ws, int64_t ws_bytes, void* stream) {
+    if (const int rc = check_linear(dtype, M, N, K)) return rc;
+    if (activation < 0 || activation >= LSDM_ACT_COUNT) return refuse(LSDM_ERR_ARG, "lsdm_linear: unknown activation %d", activation);
+    if (!x || !w || !y) return refuse(LSDM_ERR_ARG, "lsdm_linear: x, w and y must not be NULL");
+    if (ldx < K || ldw < K || (residual && ldr < N)) return refuse(LSDM_ERR_ARG, "lsdm_linear: a row stride is shorter than its row");
+    const int es = esize(dtype);
+    const bool x_ok = rows16(x, ldx, K, es), w_ok = rows16(w, ldw, K, es);
+    const Fwd f = forward_layout(dtype, M, N, K, x_ok, w_ok, ws);
+    if (f.bytes > 0 && (!ws || ws_bytes < f.bytes || !aligned16(ws)))
+        return refuse(LSDM_ERR_ARG, "lsdm_linear: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)ws_bytes, (long long)f.bytes);
+    OnDevice dev(device);
+    if (!dev.ok) return LSDM_ERR_HIP;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    GemmArgs g;
+    g.M = (int)M; g.N = (int)N; g.K = (int)K;
+    g.A = x; g.lda = ldx; g.B = w; g.ldb = ldw;
+    Epilogue& e = g.e;
+    e.bias = bias; e.bias_f32 = flags & LSDM_OP_PARAM_F32 ? 1 : 0;
+    e.res = residual; e.ldr = ldr;
+    e.out = y; e.ldo = N;
+    e.act = activation;
+    if (activation != LSDM_ACT_NONE) { e.deriv = deriv; e.ldd = N; e.deriv8 = flags & LSDM_OP_DERIV8 ? 1 : 0; }
+    e.vec = N % 8 == 0 && aligned16(y) && (!e.res || rows16(residual, ldr, N, es)) && (!e.deriv || aligned16(deriv));
+    if (f.rows) {
+        launch_rows(dtype, g, x_ok && w_ok, st);
+        return launched("lsdm_linear");
+    }
+    const int64_t kp = up(K, 8);
+    if (f.xpad) { copy_padded(dtype, x, ldx, M, K, f.x, kp, st); g.A = f.x; g.lda = kp; }
+    if (f.wpad) { copy_padded(dtype, w, ldw, N, K, f.w, kp, st); g.B = f.w; g.ldb = kp; }
+    g.part = f.part;
+    launch_gemm(dtype, f.p, g, KK, st);
+    return launched("lsdm_linear");
+}
+
+int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N, int64_t K, const void* dy, int64_t lddy, const void* deriv, const void* x,
+                         int64_t ldx, const void* codes, const void* exps, const void* w, int64_t ldw, void* dx, void* dw, void* db, void* ws,
+                         int64_t ws_bytes, void* stream) {
+    if (const int rc = check_linear(dtype, M, N, K)) return rc;
+    if (!dy || lddy < N) return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: dy must not be NULL, its row stride not shorter than a row");
+    if (dx && (!w || ldw < K)) return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: dx needs w with a row stride of at least K");
+    if (dw && !(codes ? exps != nullptr : x && ldx >= K)) return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: dw needs x (row stride of at least K) or codes with exps");
+    const int es = esize(dtype);
+    const Bwd b = backward_layout(dtype, M, N, K, dx, dw, db, deriv, codes, rows16(dy, lddy, N, es), rows16(x, ldx, K, es), rows16(w, ldw, K, es), ws);
+    if (b.bytes > 0 && (!ws || ws_bytes < b.bytes || !aligned16(ws)))
+        return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)ws_bytes, (long long)b.bytes);
+    OnDevice dev(device);
+    if (!dev.ok) return LSDM_ERR_HIP;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    // dz = dy a'(z) in the operand's type (the matrix instruction's operand) with the column sums of its fp32 values
+    const void* z = dy;
+    int64_t ldz = lddy;
+    if (b.dz || db) {
+        PrepArgs a;
+        a.src = dy; a.lds = lddy; a.deriv = deriv; a.ldv = N; a.deriv8 = deriv && (flags & LSDM_OP_DERIV8) ? 1 : 0;
+        a.rows = M; a.n = (int)N;
+        if (b.dz) { a.dst = b.z; a.ldd = b.ldz; z = b.z; ldz = b.ldz; }
+        a.part = b.cs;
+        a.vec_src = rows16(dy, lddy, 8, es);
+        a.vec_deriv = aligned16(deriv) && N % 8 == 0;
+        launch_prep(dtype, a, b.chunks, st);
+        if (db) launch_colsum_join(dtype, b.cs, b.chunks, (int)N, db, flags & LSDM_OP_PARAM_F32 ? 1 : 0, st);
+    }
+    if (dx) {
+        GemmArgs g;
+        g.M = (int)M; g.N = (int)K; g.K = (int)N;
+        g.A = z; g.lda = ldz; g.B = w; g.ldb = ldw;
+        if (b.wpad) { copy_padded(dtype, w, ldw, N, K, b.w, b.kp, st); g.B = b.w; g.ldb = b.kp; }
+        g.part = b.partx;
+        g.e.out = dx; g.e.ldo = K; g.e.vec = K % 8 == 0 && aligned16(dx);
+        launch_gemm(dtype, b.px, g, KM, st);
+    }
+    if (dw) {
+        GemmArgs g;
+        g.M = (int)N; g.N = (int)K; g.K = (int)M;
+        g.A = z; g.lda = ldz; g.B = x; g.ldb = ldx;
+        if (codes) {
+            Pack8Args a;
+            a.rows = M; a.D = (int)K; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps; a.out = b.x; a.ldo = b.kp; a.pad = (int)b.kp;
+            launch_unpack8(dtype, a, K % 32 == 0 && aligned16(codes), st);
+            g.B = b.x; g.ldb = b.kp;
+        } else if (b.xpad) {
+            copy_padded(dtype, x, ldx, M, K, b.x, b.kp, st);
+            g.B = b.x; g.ldb = b.kp;
+        }
+        g.part = b.partw;
+        g.e.out = dw; g.e.ldo = K; g.e.vec = K % 8 == 0 && aligned16(dw);
+        launch_gemm(dtype, b.pw, g, MM, st);
+    }
+    return launched("lsdm_linear_backward");
+}
+
+int64_t lsdm_layer_norm_workspace(int64_t rows, int64_t D) {
+    if (rows < 1 || D < 1 || D > kNormMaxWidth) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm: rows >= 1 and a width in [1, %d] are needed", kNormMaxWidth);
+    // (either variant's grid; the larger one)
+    const int64_t g1 = norm_grid(rows, (int)D, true, true), g2 = norm_grid(rows, (int)D, false, true);
+    return (g1 > g2 ? g1 : g2) * 2 * D * 4;
+}
+
+static int check_norm(const char* who, int dtype, int64_t rows, int64_t D) {
+    if (!dtype_ok(dtype)) return refuse(LSDM_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (rows < 1 || D < 1 || D > kNormMaxWidth) return refuse(LSDM_ERR_ARG, "%s: rows >= 1 and a width in [1, %d] are needed", who, kNormMaxWidth);
+    return LSDM_OK;
+}
+
+int lsdm_layer_norm(int device, int dtype, int flags, int64_t rows, int64_t D, const void* x, int64_t ldx, const void* w, const void* b, float eps, void* y,
+                    float* mean, float* rstd, void* codes, void* exps, void* stream) {
+    if (const int rc = check_norm("lsdm_layer_norm", dtype, rows, D)) return rc;
+    if (!x || !y || ldx < D) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm: x and y must not be NULL, the row stride not shorter than a row");
+    if ((codes == nullptr) != (exps == nullptr)) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm: codes and exps come together");
+    if (!(eps >= 0.0f)) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm: eps must be >= 0");
+    OnDevice dev(device);
+    if (!dev.ok) return LSDM_ERR_HIP;
+    NormArgs a;
+    a.rows = rows; a.D = (int)D; a.eps = eps; a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.param_f32 = flags & LSDM_OP_PARAM_F32 ? 1 : 0;
+    a.y = y; a.mean = mean; a.rstd = rstd; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps;
+    const int es = esize(dtype);
+    const bool vec = D % 8 == 0 && rows16(x, ldx, D, es) && aligned16(y) && aligned16(codes);
+    launch_norm(dtype, a, vec, norm_grid(rows, (int)D, vec, false), false, static_cast<hipStream_t>(stream));
+    return launched("lsdm_layer_norm");
+}
+
+int lsdm_layer_norm_backward(int device, int dtype, int flags, int64_t rows, int64_t D, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* codes,
+                             const void* exps, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db, void* ws, int64_t ws_bytes,
+                             void* stream) {
+    if (const int rc = check_norm("lsdm_layer_norm_backward", dtype, rows, D)) return rc;
+    if (!dy || lddy < D || !rstd) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm_backward: dy and rstd must not be NULL, the row stride not shorter than a row");
+    if (!(codes ? exps != nullptr : x && mean && ldx >= D)) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm_backward: x with mean, or codes with exps, are needed");
+    const bool part = dw || db;
+    const int64_t need = part ? lsdm_layer_norm_workspace(rows, D) : 0;
+    if (part && (!ws || ws_bytes < need || !aligned16(ws)))
+        return refuse(LSDM_ERR_ARG, "lsdm_layer_norm_backward: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)ws_bytes, (long long)need);
+    OnDevice dev(device);
+    if (!dev.ok) return LSDM_ERR_HIP;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    NormArgs a;
+    a.rows = rows; a.D = (int)D; a.x = codes ? nullptr : x; a.ldx = ldx; a.w = w; a.param_f32 = flags & LSDM_OP_PARAM_F32 ? 1 : 0;
+    a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.codes = (signed char*)codes; a.exps = (unsigned char*)exps;
+    a.dy = dy; a.lddy = lddy; a.dx = dx; a.part = part ? static_cast<float*>(ws) : nullptr;
+    const int es = esize(dtype);
+    const bool vec = D % 8 == 0 && rows16(dy, lddy, D, es) && (codes ? aligned16(codes) : rows16(x, ldx, D, es)) && (!dx || aligned16(dx));
+    const int grid = norm_grid(rows, (int)D, vec, true);
+    launch_norm(dtype, a, vec, grid, true, st);
+    if (part) launch_norm_join(dtype, a.part, grid, (int)D, dw, db, a.param_f32, st);
+    return launched("lsdm_layer_norm_backward");
+}
+
+int lsdm_pack8(int device, int dtype, int64_t rows, int64_t D, const void* x, int64_t ldx, void* codes, void* exps, void* stream) {
+    if (!dtype_ok(dtype) || rows < 1 || D < 1 || D > kMaxSize || !x || !codes || !exps || ldx < D) return refuse(LSDM_ERR_ARG, "lsdm_pack8: bad argument");
+    OnDevice dev(device);
+    if (!dev.ok) return LSDM_ERR_HIP;
+    Pack8Args a;
+    a.rows = rows; a.D = (int)D; a.x = x; a.ldx = ldx; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps;
+    launch_pack8(dtype, a, D % 32 == 0 && rows16(x, ldx, D, esize(dtype)) && aligned16(codes), static_cast<hipStream_t>(stream));
+    return launched("lsdm_pack8");
+}
+
+int lsdm_unpack8(int device, int dtype, int64_t rows, int64_t D, const void* codes, const void* exps, void* out, void* stream) {
+    if (!dtype_ok(dtype) || rows < 1 || D < 1 || D > kMaxSize || !codes || !exps || !out) return refuse(LSDM_ERR_ARG, "lsdm_unpack8: bad argument");
+    OnDevice dev(device);
+    if (!dev.ok) return LSDM_ERR_HIP;
+    Pack8Args a;
+    a.rows = rows; a.D = (int)D; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps; a.out = out; a.ldo = D;
+    launch_unpack8(dtype, a, D % 32 == 0 && aligned16(out) && aligned16(codes), static_cast<hipStream_t>(stream));
+    return launched("lsdm_unpack8");
+}
+
+}  // extern "C"

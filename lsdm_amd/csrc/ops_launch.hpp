@@ -1,0 +1,52 @@
+// Launchers of the public operators' kernels (host side of ops_gemm.hip, ops_norm.hip, ops_pack8.hip).
+#pragma once
+#include <type_traits>
+
+#include "ops.hpp"
+
+namespace lsdm {
+namespace ops {
+
+constexpr int kNormMaxWidth = 16384;      // (1024 threads, 16 values each)
+
+struct GemmPlan { int tile = 0, tiles_m = 0, tiles_n = 0, splits = 1, kchunk = 0; };
+
+struct PrepArgs {
+    const void* src = nullptr; long long lds = 0;
+    const void* deriv = nullptr; long long ldv = 0; int deriv8 = 0;
+    void* dst = nullptr; long long ldd = 0;          // NULL: only the column sums; ldd a multiple of 8 elements, rows 16-byte aligned
+    float* part = nullptr;                           // (chunks, n) column sums, or NULL
+    long long rows = 0; int n = 0;
+    int vec_src = 0, vec_deriv = 0;                  // whole 8-element pieces may be read with vector loads
+};
+
+struct NormArgs {
+    long long rows = 0; int D = 0; float eps = 0.0f;
+    const void* x = nullptr; long long ldx = 0;
+    const void *w = nullptr, *b = nullptr; int param_f32 = 0;
+    void* y = nullptr;                               // (rows, D) dense
+    float *mean = nullptr, *rstd = nullptr;          // (rows)
+    signed char* codes = nullptr; unsigned char* exps = nullptr;      // 8-bit checkpoint of h: written by the forward pass, read by the backward
+    const void* dy = nullptr; long long lddy = 0;
+    void* dx = nullptr;                              // (rows, D) dense, or NULL
+    float* part = nullptr;                           // (grid, 2, D) partial sums of dw and db, or NULL
+};
+struct Pack8Args {
+    long long rows = 0; int D = 0;
+    const void* x = nullptr; long long ldx = 0;
+    signed char* codes = nullptr; unsigned char* exps = nullptr;      // (rows, D), (rows, ceil(D / 32))
+    void* out = nullptr; long long ldo = 0; int pad = 0;              // columns D .. pad - 1 of out are zeroed
+};
+
+void launch_gemm(int dtype, const GemmPlan& p, const GemmArgs& g, int layout, hipStream_t st);
+void launch_rows(int dtype, const GemmArgs& g, bool aligned, hipStream_t st);
+void launch_prep(int dtype, const PrepArgs& a, int chunks, hipStream_t st);
+void launch_colsum_join(int dtype, const float* part, int chunks, int n, void* out, int out_f32, hipStream_t st);
+void launch_norm(int dtype, const NormArgs& a, bool vec, int grid, bool backward, hipStream_t st);
+void launch_norm_join(int dtype, const float* part, int groups, int D, void* dw, void* db, int param_f32, hipStream_t st);
+int norm_rows_per_group(int D, bool vec);            // rows a work-group of the norm kernels has in flight
+void launch_pack8(int dtype, const Pack8Args& a, bool wide, hipStream_t st);
+void launch_unpack8(int dtype, const Pack8Args& a, bool wide, hipStream_t st);
+
+}  // namespace ops
+}  // namespace lsdm
