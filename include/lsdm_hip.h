@@ -239,7 +239,7 @@ typedef enum {
 } lsdm_activation;
 enum {
     LSDM_OP_PARAM_F32 = 1,  /* bias / norm weight and bias (and their gradients) are fp32; otherwise of the call's dtype */
-    LSDM_OP_DERIV8 = 2,     /* `deriv` holds 8-bit codes u = rint(192 a'(z)) + 32 (255: NaN) instead of the call's dtype */
+    LSDM_OP_DERIV8 = 2,     /* `deriv` holds 8-bit codes u = rint(192 a'(z)) + 32 (255: NaN) instead of its wider form    */
     /* lsdm_linear_workspace only: what the call will do and which rows are not made of whole, aligned 16-byte pieces */
     LSDM_OP_BACKWARD = 4, LSDM_OP_DX = 8, LSDM_OP_DW = 16, LSDM_OP_DB = 32, LSDM_OP_DERIV = 64, LSDM_OP_CODES = 128,
     LSDM_OP_X_UNALIGNED = 256, LSDM_OP_W_UNALIGNED = 512, LSDM_OP_DY_UNALIGNED = 1024
@@ -247,7 +247,7 @@ enum {
 
 /* y = a(x w^T + bias) + residual.  x (M,K) with row stride ldx, w (N,K) with row stride ldw, bias (N) or NULL, residual (M,N) with row stride
  * ldr or NULL (it may be y itself), y (M,N) dense.  deriv: NULL, or (M,N) that receives a'(z) for lsdm_linear_backward (untouched without an
- * activation).  1 <= M, N, K <= 2^30. */
+ * activation): fp32 in fp32 calls, a 16-bit form (sign, 3 exponent bits, 12 mantissa bits) in bf16 / fp16 calls, or LSDM_OP_DERIV8's bytes.  1 <= M, N, K <= 2^30. */
 LSDM_API int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
                 int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, void* deriv, void* ws, int64_t ws_bytes, void* stream);
 /* dz = dy a'(z);  dx = dz w,  dw = dz^T x,  db = column sums of dz (each NULL: not wanted; the residual's gradient is dy).  dy (M,N) with row

@@ -4,6 +4,8 @@ The product path has no fallback: if the shared library is missing or no HIP dev
 constructors below raise ``LsdmError`` -- nothing here ever routes to a CPU implementation.
 """
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -81,6 +83,24 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_torch_ops = None
+
+
+def load_torch_ops():
+    """Loads _torch_ops.so, the tensor front end of the public operators (csrc/torch_ops.cpp; built with the library)."""
+    global _torch_ops
+    if _torch_ops is None:
+        load()
+        path = os.path.join(_HERE, "_torch_ops.so")
+        if not os.path.exists(path):
+            raise LsdmError("_torch_ops.so not found at %s -- build it with `make -C lsdm_amd/csrc` (the operators have no other front end)" % path)
+        loader = importlib.machinery.ExtensionFileLoader("_torch_ops", path)
+        module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_torch_ops", loader, origin=path))
+        loader.exec_module(module)
+        _torch_ops = module
+    return _torch_ops
 
 
 class Context:

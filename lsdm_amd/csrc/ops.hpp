@@ -104,15 +104,28 @@ __device__ __forceinline__ void act_eval(int act, float z, bool want, float& y, 
     }
 }
 
-// a'(z) in 8 bits: u = rint(192 a') + 32.  Every derivative above lies in [-0.13, 1.13], i.e. codes 7 .. 249; 0 and 1 (relu) are exact; the
-// error is at most 1/384.  Code 255 stands for NaN.
-__device__ __forceinline__ unsigned deriv_code(float d) {
+// a'(z) is kept for the backward pass in 16 bits (bf16 and fp16 calls; fp32 calls keep fp32): sign, 3 exponent bits, 12 mantissa bits.  Every derivative
+// above lies in [-0.13, 1.13], so bf16's 8 or fp16's 5 exponent bits would be wasted: this form rounds by 2^-13 relative from 2^-6 up and by 2^-19
+// absolute below, a sixteenth (bf16) and a quarter (fp16) of the type's own rounding.  The bits are fp32's after a scaling by 2^-120, which makes
+// the exponent field of [1, 2) a 7.  0x7fff stands for NaN.
+__device__ __forceinline__ unsigned deriv_code16(float d) {
+    const unsigned b = __builtin_bit_cast(unsigned, fabsf(d) * 0x1p-120f), s = (__builtin_bit_cast(unsigned, d) >> 16) & 0x8000u;
+    return d != d ? 0x7fffu : (s | (b + 0x3ffu + ((b >> 11) & 1u)) >> 11);
+}
+__device__ __forceinline__ float deriv_value16(unsigned u) {
+    const float v = __builtin_bit_cast(float, (u & 0x7fffu) << 11) * 0x1p120f;
+    return (u & 0x7fffu) == 0x7fffu ? __builtin_nanf("") : __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) | (u & 0x8000u) << 16);
+}
+// ... or, with an 8-bit checkpoint, in 8 bits: u = rint(192 a') + 32, codes 7 .. 249; 0 and 1 (relu) are exact, the error is at most 1/384.  Code 255
+// stands for NaN.
+__device__ __forceinline__ unsigned deriv_code8(float d) {
     const float u = fminf(fmaxf(rintf(192.0f * d) + 32.0f, 0.0f), 254.0f);
     return d != d ? 255u : (unsigned)u;
 }
-__device__ __forceinline__ float deriv_value(unsigned u) {
+__device__ __forceinline__ float deriv_value8(unsigned u) {
     return u == 255u ? __builtin_nanf("") : (float)((int)u - 32) * (1.0f / 192.0f);
 }
+enum DerivForm { DERIV_NONE = 0, DERIV_F32 = 1, DERIV_16 = 2, DERIV_8 = 3 };
 
 // ---- 8-bit checkpoint: groups of kGroup8 consecutive values of a row share a power-of-two step 2^e ----
 // m = max |x| of the group, e = max(floor(log2 m) - 6, -126), q = clamp(rint(x 2^-e), +-127); stored: q (int8), e + 127 (uint8), 255 for a
@@ -137,7 +150,7 @@ struct Epilogue {
     const void* bias = nullptr; int bias_f32 = 0;
     const void* res = nullptr; long long ldr = 0;
     void* out = nullptr; long long ldo = 0;
-    void* deriv = nullptr; long long ldd = 0; int deriv8 = 0;      // a'(z) for the backward pass, in the operand's type or as a code byte
+    void* deriv = nullptr; long long ldd = 0; int form = DERIV_NONE;   // a'(z) for the backward pass
     int act = OP_NONE;
     int vec = 0;                                                    // every row piece of 8 outputs is whole and 16-byte aligned
 };
@@ -148,6 +161,9 @@ struct GemmArgs {
     int tiles_m = 0, tiles_n = 0, splits = 1, kchunk = 0;
     float* part = nullptr;                                          // splits > 1: (splits, M, N) partial sums
     Epilogue e;
+    // work-groups behind the tiles' join column sums left by an earlier launch: out[c] = sum over the chunks of cs_part[chunk][c], in order
+    int blocks = 0;                                                 // work-groups of the product itself
+    const float* cs_part = nullptr; int cs_chunks = 0, cs_n = 0, cs_f32 = 0; void* cs_out = nullptr;
 };
 
 enum Layout { KK = 0, KM = 1, MM = 2 };                             // contraction axis contiguous in (A and B), (A only), (neither)

@@ -45,6 +45,7 @@ int launched(const char* what) {
 
 constexpr int64_t kMaxSize = (int64_t)1 << 30;
 constexpr int kCUs = 256;                         // MI355X
+constexpr int64_t kMaxTiles = (int64_t)1 << 30;   // work-groups of a launch
 int esize(int dtype) { return dtype == LSDM_F32 ? 4 : 2; }
 bool dtype_ok(int d) { return d == LSDM_F32 || d == LSDM_BF16 || d == LSDM_F16; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -63,29 +64,34 @@ struct Carve {
     }
 };
 
-// Tile and split of C (M, N) with contraction K.  A launch costs its rounds of work-groups (256 CUs x resident work-groups) times the steps a
-// work-group walks; the estimate below is that product with the measured time of a step, plus the join of a split contraction (its partial
-// sums are written and read once).
+// Tile and split of C (M, N) with contraction K, by an estimate of the launch's time.  A tile kind keeps up to `resident` work-groups on a CU; a
+// 128-byte step of the contraction takes max(alone, shared * n) us with n of them there, prologue and epilogue fixed + each * n us.  The grid runs
+// in full rounds of 256 `resident` work-groups and a last, thinner one; a split contraction adds the join's launch and its traffic (the partial sums
+// are written once and read once).  The constants are fitted to 1400 timed launches (135 shapes log-uniform over 16 .. 16384, every tile, 1 .. 32
+// splits, three operand layouts): the estimate's choice is within 1 % of the best one in the mean, within 16 % at worst.
+struct TileCost { int tile, resident; float alone, shared, fixed, each; };
+const TileCost kHalfTiles[] = {{256, 1, 0.0f, 1.44f, 8.8f, 0.6f}, {128, 2, 0.68f, 0.40f, 2.1f, 1.55f}, {64, 5, 0.31f, 0.18f, 2.7f, 0.07f}};
+const TileCost kSingleTiles[] = {{128, 2, 0.40f, 1.61f, 4.9f, 0.13f}, {64, 4, 0.52f, 0.49f, 0.06f, 0.09f}};
+constexpr float kJoinLaunch = 2.6f, kJoinBytesPerUs = 3.6e6f;
+
 GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
-    struct Kind { int tile, resident; float step, fixed; };        // us per 128-byte step with `resident` work-groups on a CU; prologue + epilogue
-    static const Kind half[] = {{256, 1, 1.05f, 6.0f}, {128, 2, 0.60f, 4.5f}, {64, 3, 0.45f, 3.5f}};
-    static const Kind single[] = {{128, 2, 3.6f, 6.0f}, {64, 3, 1.6f, 4.0f}};
-    const int bk = 128 / esize(dtype);
+    const bool f32 = dtype == LSDM_F32;
+    const int bk = f32 ? 32 : 64, kinds = f32 ? 2 : 3;
     const int64_t steps = (K + bk - 1) / bk;
     GemmPlan best;
     float best_us = 0.0f;
-    const Kind* kinds = dtype == LSDM_F32 ? single : half;
-    const int nk = dtype == LSDM_F32 ? 2 : 3;
-    for (int i = 0; i < nk; ++i) {
-        const Kind& k = kinds[i];
-        const int64_t tm = (M + k.tile - 1) / k.tile, tn = (N + k.tile - 1) / k.tile, tiles = tm * tn;
+    for (int i = 0; i < kinds; ++i) {
+        const TileCost& k = f32 ? kSingleTiles[i] : kHalfTiles[i];
+        const int64_t tm = (M + k.tile - 1) / k.tile, tn = (N + k.tile - 1) / k.tile;
+        if (tm * tn > kMaxTiles) continue;
         for (int s = 1; s <= 32; s = s < 4 ? s + 1 : s * 2) {
-            if (s > 1 && steps < 2 * s) break;
-            const int64_t per = (steps + s - 1) / s, used = steps ? (steps + per - 1) / per : 1;
-            if (used != s) continue;
-            const int64_t rounds = (tiles * s + kCUs * k.resident - 1) / (kCUs * k.resident);
-            float us = (float)rounds * ((float)per * k.step + k.fixed);
-            if (s > 1) us += 4.0f + (float)(s + 1) * (float)M * (float)N * 4.0f / 3.0e6f;
+            if (s > 1 && (steps < 2 * s || tm * tn * s > kMaxTiles)) break;
+            const int64_t per = (steps + s - 1) / s;
+            if ((steps + per - 1) / per != s) continue;
+            const int64_t groups = tm * tn * s, round = (int64_t)kCUs * k.resident, full = groups / round, rest = groups - full * round;
+            auto cost = [&](float n) { return (float)per * (k.alone > k.shared * n ? k.alone : k.shared * n) + k.fixed + k.each * n; };
+            float us = (float)full * cost((float)k.resident) + (rest ? cost((float)((rest + kCUs - 1) / kCUs)) : 0.0f);
+            if (s > 1) us += kJoinLaunch + (float)(s + 1) * (float)M * (float)N * 4.0f / kJoinBytesPerUs;
             if (best.tile == 0 || us < best_us) {
                 best_us = us;
                 best.tile = k.tile; best.tiles_m = (int)tm; best.tiles_n = (int)tn; best.splits = s; best.kchunk = (int)(per * bk);
@@ -146,12 +152,14 @@ Bwd backward_layout(int dtype, int64_t M, int64_t N, int64_t K, bool dx, bool dw
     return b;
 }
 
-void copy_padded(int dtype, const void* src, int64_t lds, int64_t rows, int64_t n, void* dst, int64_t ldd, hipStream_t st) {
-    PrepArgs a;
-    a.src = src; a.lds = lds; a.dst = dst; a.ldd = ldd; a.rows = rows; a.n = (int)n;
-    a.vec_src = rows16(src, lds, 8, esize(dtype));
-    launch_prep(dtype, a, prep_chunks(rows, ldd), st);
+// a job that copies rows of n elements into rows of ldd >= n, zero-padded
+PrepJob padded(int dtype, const void* src, int64_t lds, int64_t rows, int64_t n, void* dst, int64_t ldd) {
+    PrepJob j;
+    j.src = src; j.lds = lds; j.dst = dst; j.ldd = ldd; j.rows = rows; j.n = (int)n; j.chunks = prep_chunks(rows, ldd);
+    j.vec_src = rows16(src, lds, 8, esize(dtype));
+    return j;
 }
+int deriv_form(int dtype, int flags) { return flags & LSDM_OP_DERIV8 ? DERIV_8 : dtype == LSDM_F32 ? DERIV_F32 : DERIV_16; }
 
 int check_linear(int dtype, int64_t M, int64_t N, int64_t K) {
     if (!dtype_ok(dtype)) return refuse(LSDM_ERR_ARG, "lsdm_linear: unknown dtype %d", dtype);
@@ -189,6 +197,7 @@ int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int
     const int es = esize(dtype);
     const bool x_ok = rows16(x, ldx, K, es), w_ok = rows16(w, ldw, K, es);
     const Fwd f = forward_layout(dtype, M, N, K, x_ok, w_ok, ws);
+    if (!f.rows && !f.p.tile) return refuse(LSDM_ERR_ARG, "lsdm_linear: the result has more tiles than a launch can hold");
     if (f.bytes > 0 && (!ws || ws_bytes < f.bytes || !aligned16(ws)))
         return refuse(LSDM_ERR_ARG, "lsdm_linear: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)ws_bytes, (long long)f.bytes);
     OnDevice dev(device);
@@ -202,15 +211,18 @@ int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int
     e.res = residual; e.ldr = ldr;
     e.out = y; e.ldo = N;
     e.act = activation;
-    if (activation != LSDM_ACT_NONE) { e.deriv = deriv; e.ldd = N; e.deriv8 = flags & LSDM_OP_DERIV8 ? 1 : 0; }
+    if (activation != LSDM_ACT_NONE && deriv) { e.deriv = deriv; e.ldd = N; e.form = deriv_form(dtype, flags); }
     e.vec = N % 8 == 0 && aligned16(y) && (!e.res || rows16(residual, ldr, N, es)) && (!e.deriv || aligned16(deriv));
     if (f.rows) {
         launch_rows(dtype, g, x_ok && w_ok, st);
         return launched("lsdm_linear");
     }
     const int64_t kp = up(K, 8);
-    if (f.xpad) { copy_padded(dtype, x, ldx, M, K, f.x, kp, st); g.A = f.x; g.lda = kp; }
-    if (f.wpad) { copy_padded(dtype, w, ldw, N, K, f.w, kp, st); g.B = f.w; g.ldb = kp; }
+    PrepArgs prep;
+    int jobs = 0;
+    if (f.xpad) { prep.job[jobs++] = padded(dtype, x, ldx, M, K, f.x, kp); g.A = f.x; g.lda = kp; }
+    if (f.wpad) { prep.job[jobs++] = padded(dtype, w, ldw, N, K, f.w, kp); g.B = f.w; g.ldb = kp; }
+    if (jobs) launch_prep(dtype, prep, jobs, st);
     g.part = f.part;
     launch_gemm(dtype, f.p, g, KK, st);
     return launched("lsdm_linear");
@@ -225,47 +237,54 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
     if (dw && !(codes ? exps != nullptr : x && ldx >= K)) return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: dw needs x (row stride of at least K) or codes with exps");
     const int es = esize(dtype);
     const Bwd b = backward_layout(dtype, M, N, K, dx, dw, db, deriv, codes, rows16(dy, lddy, N, es), rows16(x, ldx, K, es), rows16(w, ldw, K, es), ws);
+    if ((dx && !b.px.tile) || (dw && !b.pw.tile)) return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: a gradient has more tiles than a launch can hold");
     if (b.bytes > 0 && (!ws || ws_bytes < b.bytes || !aligned16(ws)))
         return refuse(LSDM_ERR_ARG, "lsdm_linear_backward: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)ws_bytes, (long long)b.bytes);
     OnDevice dev(device);
     if (!dev.ok) return LSDM_ERR_HIP;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // dz = dy a'(z) in the operand's type (the matrix instruction's operand) with the column sums of its fp32 values
-    const void* z = dy;
-    int64_t ldz = lddy;
+    // one launch prepares everything: dz = dy a'(z) in the operand's type (the matrix instruction's operand) with the column sums of its fp32 values,
+    // x from its 8-bit checkpoint, and rows that need padding
+    PrepArgs prep;
+    int jobs = 0;
+    GemmArgs base;
+    const void *z = dy, *xs = x, *ws_ = w;
+    int64_t ldz = lddy, ldxs = ldx, ldws = ldw;
     if (b.dz || db) {
-        PrepArgs a;
-        a.src = dy; a.lds = lddy; a.deriv = deriv; a.ldv = N; a.deriv8 = deriv && (flags & LSDM_OP_DERIV8) ? 1 : 0;
-        a.rows = M; a.n = (int)N;
-        if (b.dz) { a.dst = b.z; a.ldd = b.ldz; z = b.z; ldz = b.ldz; }
-        a.part = b.cs;
-        a.vec_src = rows16(dy, lddy, 8, es);
-        a.vec_deriv = aligned16(deriv) && N % 8 == 0;
-        launch_prep(dtype, a, b.chunks, st);
-        if (db) launch_colsum_join(dtype, b.cs, b.chunks, (int)N, db, flags & LSDM_OP_PARAM_F32 ? 1 : 0, st);
+        PrepJob& j = prep.job[jobs++];
+        j.src = dy; j.lds = lddy; j.deriv = deriv; j.form = deriv ? deriv_form(dtype, flags) : DERIV_NONE;
+        j.rows = M; j.n = (int)N; j.chunks = b.chunks;
+        if (b.dz) { j.dst = b.z; j.ldd = b.ldz; z = b.z; ldz = b.ldz; }
+        j.part = b.cs;
+        j.vec_src = rows16(dy, lddy, 8, es);
+        j.vec_deriv = aligned16(deriv) && N % 8 == 0;
+    }
+    if (b.xpad) {
+        PrepJob& j = prep.job[jobs++];
+        j = padded(dtype, codes ? codes : x, codes ? K : ldx, M, K, b.x, b.kp);
+        if (codes) { j.exps = static_cast<const unsigned char*>(exps); j.vec_src = K % 8 == 0 && ((uintptr_t)codes & 7) == 0; }
+        xs = b.x; ldxs = b.kp;
+    }
+    if (b.wpad) { prep.job[jobs++] = padded(dtype, w, ldw, N, K, b.w, b.kp); ws_ = b.w; ldws = b.kp; }
+    if (jobs) launch_prep(dtype, prep, jobs, st);
+    if (db) { base.cs_part = b.cs; base.cs_chunks = b.chunks; base.cs_n = (int)N; base.cs_out = db; base.cs_f32 = flags & LSDM_OP_PARAM_F32 ? 1 : 0; }
+    if (!dx && !dw) {
+        if (db) launch_colsum_join(dtype, base, st);
+        return launched("lsdm_linear_backward");
     }
     if (dx) {
-        GemmArgs g;
+        GemmArgs g = base;                        // (the column sums are joined by the first product's launch)
+        base = GemmArgs();
         g.M = (int)M; g.N = (int)K; g.K = (int)N;
-        g.A = z; g.lda = ldz; g.B = w; g.ldb = ldw;
-        if (b.wpad) { copy_padded(dtype, w, ldw, N, K, b.w, b.kp, st); g.B = b.w; g.ldb = b.kp; }
+        g.A = z; g.lda = ldz; g.B = ws_; g.ldb = ldws;
         g.part = b.partx;
         g.e.out = dx; g.e.ldo = K; g.e.vec = K % 8 == 0 && aligned16(dx);
         launch_gemm(dtype, b.px, g, KM, st);
     }
     if (dw) {
-        GemmArgs g;
+        GemmArgs g = base;
         g.M = (int)N; g.N = (int)K; g.K = (int)M;
-        g.A = z; g.lda = ldz; g.B = x; g.ldb = ldx;
-        if (codes) {
-            Pack8Args a;
-            a.rows = M; a.D = (int)K; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps; a.out = b.x; a.ldo = b.kp; a.pad = (int)b.kp;
-            launch_unpack8(dtype, a, K % 32 == 0 && aligned16(codes), st);
-            g.B = b.x; g.ldb = b.kp;
-        } else if (b.xpad) {
-            copy_padded(dtype, x, ldx, M, K, b.x, b.kp, st);
-            g.B = b.x; g.ldb = b.kp;
-        }
+        g.A = z; g.lda = ldz; g.B = xs; g.ldb = ldxs;
         g.part = b.partw;
         g.e.out = dw; g.e.ldo = K; g.e.vec = K % 8 == 0 && aligned16(dw);
         launch_gemm(dtype, b.pw, g, MM, st);
@@ -343,7 +362,7 @@ int lsdm_unpack8(int device, int dtype, int64_t rows, int64_t D, const void* cod
     OnDevice dev(device);
     if (!dev.ok) return LSDM_ERR_HIP;
     Pack8Args a;
-    a.rows = rows; a.D = (int)D; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps; a.out = out; a.ldo = D;
+    a.rows = rows; a.D = (int)D; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps; a.out = out;
     launch_unpack8(dtype, a, D % 32 == 0 && aligned16(out) && aligned16(codes), static_cast<hipStream_t>(stream));
     return launched("lsdm_unpack8");
 }

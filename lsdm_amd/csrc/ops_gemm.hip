@@ -4,8 +4,8 @@
 //   dx        dz W                          A = dz, B(n, k) = W[k][n]: contiguous in A only                                               (KM)
 //   dW        dz^T x                        A(m, k) = dz[k][m], B(n, k) = x[k][n]: contiguous in neither                                  (MM)
 //
-// One tile core for all three.  A work-group owns a BM x BN tile of C and walks k in steps of 128 bytes (64 bf16 / fp16, 32 fp32): both operand
-// tiles come into LDS by LDS-DMA (16 bytes per lane, no registers), the next step's in flight while this one is multiplied.
+// One tile core for all three.  A work-group owns a BM x BN tile of C and walks k in steps of SB = 64 or 128 bytes: both operand tiles come into LDS by
+// LDS-DMA (16 bytes per lane, no registers), the next steps' in flight while this one is multiplied.
 //   16-bit: v_mfma_f32_16x16x32; a tile whose contraction axis is contiguous is read with ds_read_b128, the other kind with the transposing
 //           ds_read_b64_tr_b16, so that no operand is ever transposed in memory.
 //   fp32:   v_mfma_f32_32x32x2 (exact products, an fmaf chain).
@@ -14,6 +14,8 @@
 // LDS-DMA writes lane l's 16 bytes at base + 16 l, so the bank swizzle is put into the GLOBAL address a lane reads (src_* below) and undone by
 // the reader.  A lane whose k lies beyond the end reads 16 zero bytes (g_zero16); rows beyond the end are clamped to the last one, and their
 // results are not stored.
+#include <algorithm>
+
 #include "ops.hpp"
 #include "ops_launch.hpp"
 
@@ -28,30 +30,35 @@ template <class T> struct Mma;
 template <> struct Mma<__bf16> {
     static constexpr int F = 16;                 // rows of a fragment
     typedef bfrag frag; typedef f32x4 acc;
-    static __device__ __forceinline__ acc go(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static constexpr int KI = 1;                 // instructions per fragment
+    static __device__ __forceinline__ acc go(frag a, frag b, acc c, int) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<_Float16> {
     static constexpr int F = 16;
     typedef hfrag frag; typedef f32x4 acc;
-    static __device__ __forceinline__ acc go(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static constexpr int KI = 1;
+    static __device__ __forceinline__ acc go(frag a, frag b, acc c, int) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<float> {
     static constexpr int F = 32;
     typedef f32x4 frag; typedef f32x16 acc;      // a fragment is four k values, one per instruction
-    static __device__ __forceinline__ acc go(frag a, frag b, acc c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-        return c;
-    }
+    static constexpr int KI = 4;
+    static __device__ __forceinline__ acc go(frag a, frag b, acc c, int i) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0); }
 };
 
-constexpr int kStepBytes = 128;                  // bytes of the contraction axis per step
-
 // ---- LDS tiles ----------------------------------------------------------------------------------------------------------------
-// KMAJOR: R rows of 128 bytes, the 16-byte chunk c of row r at position c ^ swz(r).
-// else:   128 / sizeof(T) rows (one per k) of R elements; a block of 16 columns (32 bytes, 16-bit types) or 32 columns (128 bytes, fp32) b of
+// A step is SB bytes of the contraction axis.
+// KMAJOR: R rows of SB bytes, the 16-byte chunk c of row r at position c ^ swz(r).
+// else:   SB / sizeof(T) rows (one per k) of R elements; a block of 16 columns (32 bytes, 16-bit types) or 32 columns (128 bytes, fp32) b of
 //         row k at position b ^ swz(k).
-__device__ __forceinline__ int swz_k(int row) { return row & 7; }
+// ds_read_b128 takes its 64 lanes in four passes over the 64 banks: lanes 0-3, 12-15, 20-27; 4-11, 16-19, 28-31; and the same 32 lanes further.
+// The sixteen rows (fp32: chunks) of a pass fall into sixteen different 16-byte columns of the banks with these two forms (SQ_LDS_BANK_CONFLICT
+// from 50 % of the LDS cycles with r & 7 and (r >> 2) & 3 to 0).
+template <class T, int SB>
+__device__ __forceinline__ int swz_k(int r) {
+    if constexpr (SB == 64) return ((r >> 3) & 1) * 2;
+    else return ((r >> 1) & 1) * 2 | ((r >> 3) & 1) * 4 | (sizeof(T) == 4 ? (r >> 4) & 1 : 0);
+}
 template <class T, int R>
 __device__ __forceinline__ int swz_m(int k) {
     if constexpr (sizeof(T) == 4) return (k >> 2) & 1;
@@ -59,23 +66,23 @@ __device__ __forceinline__ int swz_m(int k) {
     else return ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
 }
 
-template <class T, int R, bool KMAJOR, int NW>
+template <class T, int R, bool KMAJOR, int NW, int SB>
 struct Loader {
-    static constexpr int NI = R / 8 / NW;        // wave instructions (1 KB each) per wave and step
-    static constexpr int EC = 16 / (int)sizeof(T);
-    static_assert(R % (8 * NW) == 0, "tile rows per wave");
+    static constexpr int NI = R * SB / 1024 / NW;        // wave instructions (1 KB each) per wave and step
+    static constexpr int EC = 16 / (int)sizeof(T), CPR = SB / 16;
+    static_assert(R * SB % (1024 * NW) == 0, "whole instructions per wave");
     const char* src[NI];
     int kpos[NI];                                // this lane's k within the step
     long long step;
 
     __device__ __forceinline__ void init(const void* base, long long ld, int row0, int rows, int k0, int wave, int lane) {
         const T* p = static_cast<const T*>(base);
-        step = KMAJOR ? kStepBytes : (long long)(kStepBytes / (int)sizeof(T)) * ld * (int)sizeof(T);
+        step = KMAJOR ? SB : (long long)(SB / (int)sizeof(T)) * ld * (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int q = wave * NI + i;
             if constexpr (KMAJOR) {
-                const int r = q * 8 + (lane >> 3), c = (lane & 7) ^ swz_k(r);
+                const int r = q * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ swz_k<T, SB>(r);
                 const int gr = min(row0 + r, rows - 1);
                 kpos[i] = c * EC;
                 src[i] = reinterpret_cast<const char*>(p + (long long)gr * ld + k0 + c * EC);
@@ -92,7 +99,7 @@ struct Loader {
     }
     // requests the step that starts kleft elements before the end of the contraction range
     __device__ __forceinline__ void issue(unsigned lds, int wave, int kleft) {
-        constexpr int BK = kStepBytes / (int)sizeof(T);
+        constexpr int BK = SB / (int)sizeof(T);
         if (kleft >= BK) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) lds_dma16(src[i], lds + (wave * NI + i) * 1024);
@@ -106,19 +113,19 @@ struct Loader {
 };
 
 // fragments of one wave: NF blocks of F rows starting at row0 of the tile
-template <class T, int R, bool KMAJOR, int NF>
+template <class T, int R, bool KMAJOR, int NF, int SB>
 struct Reader {
     typedef Mma<T> MM_;
     typedef typename MM_::frag frag;
     static constexpr int RB = R * (int)sizeof(T);
-    static constexpr int KS = sizeof(T) == 4 ? 4 : 2;      // sub-steps of a step (8 fp32 or 32 16-bit k each)
+    static constexpr int KS = sizeof(T) == 4 ? SB / 32 : SB / 64;      // sub-steps of a step (8 fp32 or 32 16-bit k each)
     int off[(KMAJOR && sizeof(T) == 2) || sizeof(T) == 4 ? KS : NF];
     int frow;                                              // (fp32, column tiles)
     __device__ __forceinline__ void init(int row0, int lane) {
         if constexpr (sizeof(T) == 2 && KMAJOR) {
             const int r = row0 + (lane & 15);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) off[s] = r * kStepBytes + (((s * 4 + (lane >> 4)) ^ swz_k(r)) << 4);
+            for (int s = 0; s < KS; ++s) off[s] = r * SB + (((s * 4 + (lane >> 4)) ^ swz_k<T, SB>(r)) << 4);
         } else if constexpr (sizeof(T) == 2) {
             const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
@@ -126,14 +133,14 @@ struct Reader {
         } else if constexpr (KMAJOR) {
             const int r = row0 + (lane & 31);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) off[s] = r * kStepBytes + (((2 * s + (lane >> 5)) ^ swz_k(r)) << 4);
+            for (int s = 0; s < KS; ++s) off[s] = r * SB + (((2 * s + (lane >> 5)) ^ swz_k<T, SB>(r)) << 4);
         } else {
             frow = row0;
         }
     }
     __device__ __forceinline__ frag get(const char* tile, int s, int i, int lane) const {
         if constexpr (sizeof(T) == 2 && KMAJOR) {
-            return *reinterpret_cast<const frag*>(tile + off[s] + i * 16 * kStepBytes);
+            return *reinterpret_cast<const frag*>(tile + off[s] + i * 16 * SB);
         } else if constexpr (sizeof(T) == 2) {
             typedef __attribute__((address_space(3))) s16x4* lp;
             const char* p = tile + off[i] + s * 32 * RB;
@@ -142,7 +149,7 @@ struct Reader {
             u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * RB));
             return u.f;
         } else if constexpr (KMAJOR) {
-            return *reinterpret_cast<const frag*>(tile + off[s] + i * 32 * kStepBytes);
+            return *reinterpret_cast<const frag*>(tile + off[s] + i * 32 * SB);
         } else {
             const int h = lane >> 5, b = ((frow >> 5) + i) ^ h;           // swz_m(k) = (k >> 2) & 1 = h for k = 8 s + 4 h + j
             const char* p = tile + (8 * s + 4 * h) * RB + (b << 7) + (lane & 31) * 4;
@@ -174,18 +181,28 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
 #pragma unroll
         for (int j = 0; j < 8; ++j) act_eval<T>(e.act, z[j], want, y[j], d[j]);
         if (want) {
-            if (e.deriv8) {
+            if (e.form == DERIV_8) {
                 unsigned char* p = static_cast<unsigned char*>(e.deriv) + m * e.ldd + n;
                 unsigned c[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) c[j] = deriv_code(d[j]);
+                for (int j = 0; j < 8; ++j) c[j] = deriv_code8(d[j]);
                 if (e.vec) *reinterpret_cast<u32x2*>(p) = u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
                 else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) if (j < cnt) p[j] = (unsigned char)c[j];
                 }
+            } else if constexpr (sizeof(T) == 2) {
+                unsigned short* p = static_cast<unsigned short*>(e.deriv) + m * e.ldd + n;
+                unsigned c[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) c[j] = deriv_code16(d[j]);
+                if (e.vec) *reinterpret_cast<u32x4*>(p) = u32x4{c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16};
+                else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) if (j < cnt) p[j] = (unsigned short)c[j];
+                }
             } else {
-                T* p = static_cast<T*>(e.deriv) + m * e.ldd + n;
+                float* p = static_cast<float*>(e.deriv) + m * e.ldd + n;
                 if (e.vec) store8(p, d); else store8n(p, cnt, d);
             }
         }
@@ -203,22 +220,45 @@ __device__ __forceinline__ void bias8(const Epilogue& e, int n, int N, float (&b
     for (int j = 0; j < 8; ++j) b[j] = e.bias && n + j < N ? param<T>(e.bias, e.bias_f32, n + j) : 0.0f;
 }
 
+// out[c] = sum over the chunks of part[chunk][c]: 64 columns per work-group, its waves take every nw-th chunk, joined in order
+template <class T>
+__device__ __forceinline__ void colsum_join(const GemmArgs& g, int block, float* red) {
+    const int t = threadIdx.x, c = block * 64 + (t & 63), q = t >> 6, nw = (int)blockDim.x >> 6;
+    float s = 0.0f;
+    if (c < g.cs_n)
+#pragma unroll 4
+        for (int k = q; k < g.cs_chunks; k += nw) s += g.cs_part[(long long)k * g.cs_n + c];
+    red[t] = s;
+    wg_sync();
+    if (q == 0 && c < g.cs_n) {
+        for (int k = 1; k < nw; ++k) s += red[k * 64 + t];
+        store_param<T>(g.cs_out, g.cs_f32, c, s);
+    }
+}
+template <class T>
+__global__ __launch_bounds__(256) void colsum_join_kernel(GemmArgs g) {
+    __shared__ float red[256];
+    colsum_join<T>(g, (int)blockIdx.x, red);
+}
+
 // ---- the tile kernel ------------------------------------------------------------------------------------------------------------
-template <class T, int BM, int BN, int WGM, int WGN, int STAGES, bool AKM, bool BKM, int WPE>
+template <class T, int BM, int BN, int WGM, int WGN, int STAGES, int SB, bool AKM, bool BKM, int WPE>
 __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
     typedef Mma<T> MM_;
     constexpr int NW = WGM * WGN, TM = BM / WGM, TN = BN / WGN, F = MM_::F, FM = TM / F, FN = TN / F;
-    constexpr int BK = kStepBytes / (int)sizeof(T), KS = sizeof(T) == 4 ? 4 : 2;
-    constexpr int TA = BM * kStepBytes, TB = BN * kStepBytes, ST = TA + TB;
+    constexpr int BK = SB / (int)sizeof(T), KS = Reader<T, BM, AKM, FM, SB>::KS;
+    constexpr int TA = BM * SB, TB = BN * SB, ST = TA + TB;
     constexpr int RW = TM < 64 ? TM : 64, PITCH = TN * 4 + 16, EPI = RW * PITCH;        // epilogue: RW rows of a wave's tile at a time, in fp32
     constexpr int BYTES = ST * STAGES > EPI * NW ? ST * STAGES : EPI * NW;
     __shared__ __attribute__((aligned(1024))) char lds[BYTES];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave / WGN, wn = wave - wm * WGN;
 
+    if ((int)blockIdx.x >= g.blocks) { colsum_join<T>(g, (int)blockIdx.x - g.blocks, reinterpret_cast<float*>(lds)); return; }
+
     // tiles in groups of 8 rows of tiles, an XCD walks a contiguous range: the tiles in flight on an XCD share their operands in its L2
     const int tiles = g.tiles_m * g.tiles_n;
-    int v = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+    int v = xcd_remap((int)blockIdx.x, g.blocks);
     const int ks = v / tiles;
     v -= ks * tiles;
     const int per = 8 * g.tiles_n, grp = v / per, gm = min(8, g.tiles_m - grp * 8), in = v - grp * per;
@@ -227,12 +267,12 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
     const int k_lo = ks * g.kchunk, k_hi = min(g.K, k_lo + g.kchunk);
     const int nk = k_hi > k_lo ? (k_hi - k_lo + BK - 1) / BK : 0;
 
-    Loader<T, BM, AKM, NW> la;
-    Loader<T, BN, BKM, NW> lb;
+    Loader<T, BM, AKM, NW, SB> la;
+    Loader<T, BN, BKM, NW, SB> lb;
     la.init(g.A, g.lda, m0, g.M, k_lo, wave, lane);
     lb.init(g.B, g.ldb, n0, g.N, k_lo, wave, lane);
-    Reader<T, BM, AKM, FM> ra;
-    Reader<T, BN, BKM, FN> rb;
+    Reader<T, BM, AKM, FM, SB> ra;
+    Reader<T, BN, BKM, FN, SB> rb;
     ra.init(wm * TM, lane);
     rb.init(wn * TN, lane);
     const unsigned base = lds_addr(lds);
@@ -253,20 +293,24 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
             lb.issue(base + s * ST + TA, wave, k_hi - k_lo - issued * BK);
             ++issued;
         }
+    constexpr int PER = Loader<T, BM, AKM, NW, SB>::NI + Loader<T, BN, BKM, NW, SB>::NI;      // LDS-DMA instructions per wave and step
+    auto issue_next = [&](int buf) {
+        la.issue(base + buf * ST, wave, k_hi - k_lo - issued * BK);
+        lb.issue(base + buf * ST + TA, wave, k_hi - k_lo - issued * BK);
+        ++issued;
+    };
+    // waits until at most `younger` steps' pieces of this wave are in flight
+    auto wait_landed = [&](int younger) {
+        if (younger <= 0) lds_dma_wait();
+        else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+    };
     int buf = 0;
     for (int it = 0; it < nk; ++it) {
         // this step's pieces have landed (the younger steps' may still be on their way), for every wave behind the barrier
-        constexpr int PER = Loader<T, BM, AKM, NW>::NI + Loader<T, BN, BKM, NW>::NI;
-        if (STAGES == 2 || issued == it + 1) lds_dma_wait();
-        else if (STAGES == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wait_landed(min(issued - it - 1, STAGES - 2));
         wg_sync();
-        if (issued < nk) {       // into the buffer of step it - 1, which every wave has read
-            const int nb = buf + STAGES - 1 >= STAGES ? buf - 1 : buf + STAGES - 1;
-            la.issue(base + nb * ST, wave, k_hi - k_lo - issued * BK);
-            lb.issue(base + nb * ST + TA, wave, k_hi - k_lo - issued * BK);
-            ++issued;
-        }
+        if (issued < nk) issue_next(buf == 0 ? STAGES - 1 : buf - 1);       // the buffer of step it - 1, which every wave has read
         const char* ta = lds + buf * ST;
         const char* tb = ta + TA;
 #pragma unroll
@@ -277,9 +321,11 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
 #pragma unroll
             for (int i = 0; i < FM; ++i) fa[i] = ra.get(ta, s, i, lane);
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+            for (int q = 0; q < MM_::KI; ++q)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = MM_::go(fb[j], fa[i], acc[i][j]);
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = MM_::go(fb[j], fa[i], acc[i][j], q);
         }
         buf = buf + 1 == STAGES ? 0 : buf + 1;
     }
@@ -376,7 +422,7 @@ __device__ __forceinline__ typename Mma<T>::frag row_frag(const T* p, int k, int
     return f;
 }
 template <class T> struct RowMma {
-    static __device__ __forceinline__ f32x4 go(typename Mma<T>::frag a, typename Mma<T>::frag b, f32x4 c) { return Mma<T>::go(a, b, c); }
+    static __device__ __forceinline__ f32x4 go(typename Mma<T>::frag a, typename Mma<T>::frag b, f32x4 c) { return Mma<T>::go(a, b, c, 0); }
 };
 template <> struct RowMma<float> {
     static __device__ __forceinline__ f32x4 go(f32x4 a, f32x4 b, f32x4 c) {
@@ -431,38 +477,66 @@ __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs g) {
     }
 }
 
-// ---- preparation of the backward pass and of operands whose rows no 16-byte load divides ----
-// dst (rows, ldd) = src (rows, n) * d, columns n .. ldd - 1 zero.  deriv: 0 none, 1 of type T, 2 code bytes.
-// COLSUM: part[blockIdx.y][c] = the work-group's sum of the products over its rows (fp32, in row order per thread, joined in a fixed order)
+// ---- what the products need prepared, up to three jobs in one launch (blockIdx.z) ----
+//   dst (rows, ldd) = src (rows, n) * d, or the values of an 8-bit checkpoint; columns n .. ldd - 1 are zeroed, so that rows no 16-byte load divides
+//   become rows that one does.  part[blockIdx.y][c] = the work-group's sum of the fp32 products over its rows (a fixed order).
+// Bound by HBM: each operand is read once, dst is written once.
 template <class T>
-__global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
+__global__ __launch_bounds__(256) void prep_kernel(PrepArgs args) {
+    const PrepJob& a = args.job[blockIdx.z];
     __shared__ float red[8][256 + 8];
     const int t = threadIdx.x, tc = t & 31, tr = t >> 5;
     const int c0 = ((int)blockIdx.x * 32 + tc) * 8;
-    const long long per = (a.rows + gridDim.y - 1) / gridDim.y, lo = (long long)blockIdx.y * per, hi = min(a.rows, lo + per);
-    const int n = min(8, a.n - c0);
+    if ((int)blockIdx.y >= a.chunks || (long long)blockIdx.x * 256 >= (a.dst && a.ldd > a.n ? a.ldd : a.n)) return;      // (whole work-groups)
+    const long long per = (a.rows + a.chunks - 1) / a.chunks, lo = (long long)blockIdx.y * per, hi = min(a.rows, lo + per);
+    const int n = max(0, min(8, a.n - c0));
+    const int gpr = (a.n + 31) >> 5;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c0 < a.ldd || n > 0) {
+    if (n > 0 || (a.dst && c0 < a.ldd)) {
 #pragma unroll 2
         for (long long r = lo + tr; r < hi; r += 8) {
             float v[8], d[8];
-            const T* p = static_cast<const T*>(a.src) + r * a.lds + c0;
-            if (a.vec_src && n == 8) load8(p, v); else load8n(p, n, v);
-            if (a.deriv8) {
-                const unsigned char* q = static_cast<const unsigned char*>(a.deriv) + r * a.ldv + c0;
-                if (a.vec_deriv && n == 8) {
+            if (a.exps) {
+                const signed char* q = static_cast<const signed char*>(a.src) + r * a.n + c0;
+                const float step = n > 0 ? exp8_step(a.exps[r * gpr + (c0 >> 5)]) : 0.0f;
+                if (a.vec_src && n == 8) {
                     const u32x2 w = *reinterpret_cast<const u32x2*>(q);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) d[j] = deriv_value((w[j >> 2] >> (8 * (j & 3))) & 255u);
+                    for (int j = 0; j < 8; ++j) v[j] = (float)((int)(w[j >> 2] << (24 - 8 * (j & 3))) >> 24) * step;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value(q[j]) : 0.0f;
+                    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)q[j] * step : 0.0f;
                 }
-            } else if (a.deriv) {
-                const T* q = static_cast<const T*>(a.deriv) + r * a.ldv + c0;
-                if (a.vec_deriv && n == 8) load8(q, d); else load8n(q, n, d);
+            } else {
+                const T* p = static_cast<const T*>(a.src) + r * a.lds + c0;
+                if (a.vec_src && n == 8) load8(p, v); else load8n(p, n, v);
             }
-            if (a.deriv) {
+            if (a.form != DERIV_NONE) {
+                const long long at = r * a.n + c0;
+                if (a.form == DERIV_8) {
+                    const unsigned char* q = static_cast<const unsigned char*>(a.deriv) + at;
+                    if (a.vec_deriv) {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(q);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[j] = deriv_value8((w[j >> 2] >> (8 * (j & 3))) & 255u);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value8(q[j]) : 0.0f;
+                    }
+                } else if constexpr (sizeof(T) == 2) {
+                    const unsigned short* q = static_cast<const unsigned short*>(a.deriv) + at;
+                    if (a.vec_deriv) {
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(q);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[j] = deriv_value16((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value16(q[j]) : 0.0f;
+                    }
+                } else {
+                    const float* q = static_cast<const float*>(a.deriv) + at;
+                    if (a.vec_deriv) load8(q, d); else load8n(q, n, d);
+                }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] * d[j] : 0.0f;
             }
@@ -484,29 +558,15 @@ __global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
     }
 }
 
-// out[c] = sum over the chunks of part[chunk][c], in order
-template <class T>
-__global__ __launch_bounds__(256) void colsum_join_kernel(const float* __restrict__ part, int chunks, int n, void* out, int out_f32) {
-    __shared__ float red[4][64];
-    const int c = (int)blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    float s = 0.0f;
-    if (c < n)
-#pragma unroll 4
-        for (int k = q; k < chunks; k += 4) s += part[(long long)k * n + c];
-    red[q][threadIdx.x & 63] = s;
-    wg_sync();
-    if (q == 0 && c < n) store_param<T>(out, out_f32, c, (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
-}
-
 // ---- host side ------------------------------------------------------------------------------------------------------------------
 namespace {
 
-template <class T, int BM, int BN, int WGM, int WGN, int STAGES, int WPE>
+template <class T, int BM, int BN, int WGM, int WGN, int STAGES, int SB, int WPE>
 void launch_layout(const GemmArgs& g, int layout, unsigned grid, hipStream_t st) {
     const dim3 b(64 * WGM * WGN);
-    if (layout == KK) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, true, true, WPE>), dim3(grid), b, 0, st, g);
-    else if (layout == KM) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, true, false, WPE>), dim3(grid), b, 0, st, g);
-    else hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, false, false, WPE>), dim3(grid), b, 0, st, g);
+    if (layout == KK) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, SB, true, true, WPE>), dim3(grid), b, 0, st, g);
+    else if (layout == KM) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, SB, true, false, WPE>), dim3(grid), b, 0, st, g);
+    else hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, SB, false, false, WPE>), dim3(grid), b, 0, st, g);
 }
 
 }  // namespace
@@ -514,12 +574,13 @@ void launch_layout(const GemmArgs& g, int layout, unsigned grid, hipStream_t st)
 template <class T>
 void launch_gemm_t(const GemmPlan& p, GemmArgs g, int layout, hipStream_t st) {
     g.tiles_m = p.tiles_m; g.tiles_n = p.tiles_n; g.splits = p.splits; g.kchunk = p.kchunk;
-    const unsigned grid = (unsigned)((long long)p.tiles_m * p.tiles_n * p.splits);
+    g.blocks = p.tiles_m * p.tiles_n * p.splits;
+    const unsigned grid = (unsigned)(g.blocks + (g.cs_out ? (g.cs_n + 63) / 64 : 0));
     if constexpr (sizeof(T) == 2) {
-        if (p.tile == 256) launch_layout<T, 256, 256, 2, 4, 2, 2>(g, layout, grid, st);
+        if (p.tile == 256) launch_layout<T, 256, 256, 2, 4, 2, 128, 2>(g, layout, grid, st);
     }
-    if (p.tile == 128) launch_layout<T, 128, 128, 2, 2, 2, 2>(g, layout, grid, st);
-    else if (p.tile == 64) launch_layout<T, 64, 64, 2, 2, 3, 2>(g, layout, grid, st);
+    if (p.tile == 128) launch_layout<T, 128, 128, 2, 2, 2, 128, 2>(g, layout, grid, st);
+    else if (p.tile == 64) launch_layout<T, 64, 64, 2, 2, 2, 128, 2>(g, layout, grid, st);
     if (p.splits > 1) {
         const int ppr = (g.N + 7) / 8;
         const long long pieces = (long long)g.M * ppr;
@@ -559,18 +620,23 @@ void launch_rows(int dtype, const GemmArgs& g, bool aligned, hipStream_t st) {
     else if (dtype == 1) launch_rows_t<__bf16>(g, aligned, st);
     else launch_rows_t<_Float16>(g, aligned, st);
 }
-void launch_prep(int dtype, const PrepArgs& a, int chunks, hipStream_t st) {
-    const long long cols = a.ldd > a.n ? a.ldd : a.n;
-    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)chunks);
+void launch_prep(int dtype, const PrepArgs& a, int jobs, hipStream_t st) {
+    unsigned x = 1, y = 1;
+    for (int i = 0; i < jobs; ++i) {
+        const long long cols = a.job[i].ldd > a.job[i].n ? a.job[i].ldd : a.job[i].n;
+        x = std::max(x, (unsigned)((cols + 255) / 256));
+        y = std::max(y, (unsigned)a.job[i].chunks);
+    }
+    const dim3 grid(x, y, (unsigned)jobs);
     if (dtype == 0) hipLaunchKernelGGL((prep_kernel<float>), grid, dim3(256), 0, st, a);
     else if (dtype == 1) hipLaunchKernelGGL((prep_kernel<__bf16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((prep_kernel<_Float16>), grid, dim3(256), 0, st, a);
 }
-void launch_colsum_join(int dtype, const float* part, int chunks, int n, void* out, int out_f32, hipStream_t st) {
-    const dim3 grid((unsigned)((n + 63) / 64));
-    if (dtype == 0) hipLaunchKernelGGL((colsum_join_kernel<float>), grid, dim3(256), 0, st, part, chunks, n, out, out_f32);
-    else if (dtype == 1) hipLaunchKernelGGL((colsum_join_kernel<__bf16>), grid, dim3(256), 0, st, part, chunks, n, out, out_f32);
-    else hipLaunchKernelGGL((colsum_join_kernel<_Float16>), grid, dim3(256), 0, st, part, chunks, n, out, out_f32);
+void launch_colsum_join(int dtype, const GemmArgs& g, hipStream_t st) {
+    const dim3 grid((unsigned)((g.cs_n + 63) / 64));
+    if (dtype == 0) hipLaunchKernelGGL((colsum_join_kernel<float>), grid, dim3(256), 0, st, g);
+    else if (dtype == 1) hipLaunchKernelGGL((colsum_join_kernel<__bf16>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((colsum_join_kernel<_Float16>), grid, dim3(256), 0, st, g);
 }
 
 }  // namespace ops

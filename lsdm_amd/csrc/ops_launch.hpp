@@ -11,14 +11,16 @@ constexpr int kNormMaxWidth = 16384;      // (1024 threads, 16 values each)
 
 struct GemmPlan { int tile = 0, tiles_m = 0, tiles_n = 0, splits = 1, kchunk = 0; };
 
-struct PrepArgs {
+struct PrepJob {
     const void* src = nullptr; long long lds = 0;
-    const void* deriv = nullptr; long long ldv = 0; int deriv8 = 0;
+    const unsigned char* exps = nullptr;             // not NULL: src holds the codes of an 8-bit checkpoint (dense rows)
+    const void* deriv = nullptr; int form = DERIV_NONE;               // dense rows
     void* dst = nullptr; long long ldd = 0;          // NULL: only the column sums; ldd a multiple of 8 elements, rows 16-byte aligned
     float* part = nullptr;                           // (chunks, n) column sums, or NULL
-    long long rows = 0; int n = 0;
-    int vec_src = 0, vec_deriv = 0;                  // whole 8-element pieces may be read with vector loads
+    long long rows = 0; int n = 0, chunks = 1;
+    int vec_src = 0, vec_deriv = 0;                  // whole 8-element pieces may be read with vector loads (vec_deriv: all of them are whole)
 };
+struct PrepArgs { PrepJob job[3]; };
 
 struct NormArgs {
     long long rows = 0; int D = 0; float eps = 0.0f;
@@ -35,13 +37,13 @@ struct Pack8Args {
     long long rows = 0; int D = 0;
     const void* x = nullptr; long long ldx = 0;
     signed char* codes = nullptr; unsigned char* exps = nullptr;      // (rows, D), (rows, ceil(D / 32))
-    void* out = nullptr; long long ldo = 0; int pad = 0;              // columns D .. pad - 1 of out are zeroed
+    void* out = nullptr;                             // (rows, D) dense
 };
 
 void launch_gemm(int dtype, const GemmPlan& p, const GemmArgs& g, int layout, hipStream_t st);
 void launch_rows(int dtype, const GemmArgs& g, bool aligned, hipStream_t st);
-void launch_prep(int dtype, const PrepArgs& a, int chunks, hipStream_t st);
-void launch_colsum_join(int dtype, const float* part, int chunks, int n, void* out, int out_f32, hipStream_t st);
+void launch_prep(int dtype, const PrepArgs& a, int jobs, hipStream_t st);
+void launch_colsum_join(int dtype, const GemmArgs& g, hipStream_t st);
 void launch_norm(int dtype, const NormArgs& a, bool vec, int grid, bool backward, hipStream_t st);
 void launch_norm_join(int dtype, const float* part, int groups, int D, void* dw, void* db, int param_f32, hipStream_t st);
 int norm_rows_per_group(int D, bool vec);            // rows a work-group of the norm kernels has in flight

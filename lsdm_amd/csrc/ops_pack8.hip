@@ -36,17 +36,15 @@ __global__ __launch_bounds__(256) void pack8_wide_kernel(Pack8Args a, long long 
     if ((threadIdx.x & 1) == 0) a.exps[i >> 1] = (unsigned char)b;
 }
 template <class T>
-__global__ __launch_bounds__(256) void unpack8_wide_kernel(Pack8Args a, long long pieces, int ppr) {
+__global__ __launch_bounds__(256) void unpack8_wide_kernel(Pack8Args a, long long pieces) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
-    const long long r = i / ppr;
-    const int c = (int)(i - r * ppr) * 16;
     const u32x4 w = *reinterpret_cast<const u32x4*>(a.codes + i * 16);
     const float s = exp8_step(a.exps[i >> 1]);
     float v[2][8];
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k >> 3][k & 7] = (float)((int)(w[k >> 2] << (24 - 8 * (k & 3))) >> 24) * s;
-    T* p = static_cast<T*>(a.out) + r * a.ldo + c;
+    T* p = static_cast<T*>(a.out) + i * 16;
     store8(p, v[0]);
     store8(p + 8, v[1]);
 }
@@ -64,14 +62,13 @@ __global__ __launch_bounds__(256) void pack8_any_kernel(Pack8Args a, long long g
     if (c < a.D) a.codes[r * a.D + c] = (signed char)code8(x, exp8_inv(b));
     if ((threadIdx.x & 31) == 0) a.exps[g] = (unsigned char)b;
 }
-// (also writes the zero padding of a destination whose rows are longer than D)
 template <class T>
-__global__ __launch_bounds__(256) void unpack8_any_kernel(Pack8Args a, long long total, int width, int gpr) {
+__global__ __launch_bounds__(256) void unpack8_any_kernel(Pack8Args a, long long total, int gpr) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
-    const long long r = i / width;
-    const int c = (int)(i - r * width);
-    static_cast<T*>(a.out)[r * a.ldo + c] = (T)(c < a.D ? (float)a.codes[r * a.D + c] * exp8_step(a.exps[r * gpr + (c >> 5)]) : 0.0f);
+    const long long r = i / a.D;
+    const int c = (int)(i - r * a.D);
+    static_cast<T*>(a.out)[i] = (T)((float)a.codes[i] * exp8_step(a.exps[r * gpr + (c >> 5)]));
 }
 
 namespace {
@@ -85,9 +82,9 @@ void pack_t(const Pack8Args& a, bool wide, hipStream_t st) {
 }
 template <class T>
 void unpack_t(const Pack8Args& a, bool wide, hipStream_t st) {
-    const int gpr = (a.D + 31) / 32, width = a.pad > a.D ? a.pad : a.D;
-    if (wide) hipLaunchKernelGGL((unpack8_wide_kernel<T>), dim3(blocks(a.rows * (a.D / 16))), dim3(256), 0, st, a, a.rows * (a.D / 16), a.D / 16);
-    else hipLaunchKernelGGL((unpack8_any_kernel<T>), dim3(blocks(a.rows * width)), dim3(256), 0, st, a, a.rows * width, width, gpr);
+    const int gpr = (a.D + 31) / 32;
+    if (wide) hipLaunchKernelGGL((unpack8_wide_kernel<T>), dim3(blocks(a.rows * (a.D / 16))), dim3(256), 0, st, a, a.rows * (a.D / 16));
+    else hipLaunchKernelGGL((unpack8_any_kernel<T>), dim3(blocks(a.rows * a.D)), dim3(256), 0, st, a, a.rows * a.D, gpr);
 }
 }  // namespace
 
