@@ -149,17 +149,20 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_fwd_kernel(NormArgs 
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += x[i][j];
-        const float mu = row_sum2<NT>(s, 0.0f, red, t).x * inv_d;
-        float q = 0.0f;
+        // the mean's own rounding is taken out again: d = the mean of x - mu (a row without spread gives h = 0, not a last bit times 1 / sqrt(eps))
+        float mu = row_sum2<NT>(s, 0.0f, red, t).x / (float)D, q = 0.0f;
+        s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { x[i][j] = col_of<NT, VEC>(l, i, j) < D ? x[i][j] - mu : 0.0f; q = fmaf(x[i][j], x[i][j], q); }
-        const float rstd = 1.0f / sqrtf(row_sum2<NT>(q, 0.0f, red, t).x * inv_d + a.eps);
+            for (int j = 0; j < 8; ++j) { x[i][j] = col_of<NT, VEC>(l, i, j) < D ? x[i][j] - mu : 0.0f; s += x[i][j]; q = fmaf(x[i][j], x[i][j], q); }
+        const float2 c = row_sum2<NT>(s, q, red, t);
+        const float d = c.x * inv_d, rstd = 1.0f / sqrtf(fmaxf(fmaf(c.y, inv_d, -d * d), 0.0f) + a.eps);
+        mu += d;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[i][j] *= rstd;
+            for (int j = 0; j < 8; ++j) x[i][j] = col_of<NT, VEC>(l, i, j) < D ? (x[i][j] - d) * rstd : 0.0f;
         if (a.mean && l == 0) a.mean[r] = mu;
         if (a.rstd && l == 0) a.rstd[r] = rstd;
         if (a.codes) row_encode<NT, NV, VEC>(x, D, l, a.codes + r * D, a.exps + r * ((D + 31) >> 5));

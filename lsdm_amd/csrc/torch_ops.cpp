@@ -78,7 +78,8 @@ void check_capture(const char* who, const Tensor& x, std::initializer_list<const
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!node) continue;
         const auto s = node->stream();
-        if (s && s->device_index() == x.device().index() && *s != current.unwrap() && *s == c10::hip::getDefaultHIPStream(x.device().index()).unwrap())
+        // (by number: the node's stream carries the device type that torch shows, this one the runtime's)
+        if (s && s->device_index() == x.device().index() && s->id() != current.id() && s->id() == c10::hip::getDefaultHIPStream(x.device().index()).id())
             throw LsdmFailure(text(who, ": a leaf of this captured call is held by a live autograd graph that was built on the default stream; release that graph "
                                         "(or build it on a side stream) before the capture"));
     }
@@ -88,7 +89,7 @@ variable_list differentiable_once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
     for (Tensor& g : grads)
         if (g.defined()) {
-            variable_list one{g};
+            variable_list one{g.detach().set_requires_grad(true)};
             g = torch::autograd::DelayedError("the gradients of lsdm_amd.ops are differentiable once", 1).apply(std::move(one))[0];
         }
     return grads;

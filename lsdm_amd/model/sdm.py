@@ -17,6 +17,8 @@ Extensions (keyword-only, defaults preserve reference behaviour):
     "f32") selects the arithmetic of the dense 1x1-conv / Linear stacks: exact fp32 MFMA, fp32 operands split into
     bf16 hi+lo with 3 bf16 MFMAs per product (fp32-class results, same <= 1e-3 parity bar), or plain bf16 products.
     Geometry, normalisations, softmaxes and the sampler arithmetic are fp32 in every mode.
+  * ``text_kernels=True`` runs the dense layers and norms of the text tower that the model loads itself on ``lsdm_amd.ops`` (lsdm_amd/text.py); by
+    default the third-party package's eager layers run, as in the reference.
   * ``forward(..., fps_starts=...)`` injects the four FPS start draws; by default they are drawn
     from the global CPU generator exactly where the reference draws them
     (model/pcd_backbone/pointnet2_utils.py:72 -- ``torch.randint`` without a device argument).
@@ -56,6 +58,7 @@ class SceneDiffusionModel(nn.Module):
                  pcd_backbone_type="PNT2", human_backbone_type="POSA", text_encoder_type="CLIP", **kwargs):
         super().__init__()
         self.precision = kwargs.pop("precision", None) or os.environ.get("LSDM_PRECISION", "f32")
+        self.text_kernels = bool(kwargs.pop("text_kernels", False))
         if self.precision not in _lib.PRECISIONS:
             raise ValueError("precision must be one of %s" % sorted(_lib.PRECISIONS))
         if pcd_backbone_type != "PNT2" or human_backbone_type != "POSA":
@@ -162,8 +165,8 @@ class SceneDiffusionModel(nn.Module):
             feats = y
         else:
             if self.text_encoder is None:       # model/sdm.py:146-149: the encoder is chosen by text_encoder_type
-                self.text_encoder = (_default_clip_encoder(self.clip_version, device) if self.text_encoder_type == "CLIP"
-                                     else _default_bert_encoder(device))
+                self.text_encoder = (_default_clip_encoder(self.clip_version, device, self.text_kernels) if self.text_encoder_type == "CLIP"
+                                     else _default_bert_encoder(device, self.text_kernels))
             feats = self.text_encoder(list(y))
         feats = feats.to(device=device, dtype=torch.float32).contiguous()
         if feats.shape != (batch, self.clip_dim):
@@ -312,7 +315,7 @@ class SceneDiffusionModel(nn.Module):
         return out_cat, out_x0
 
 
-def _default_clip_encoder(clip_version, device):
+def _default_clip_encoder(clip_version, device, kernels=False):
     """CLIP text tower as the reference uses it (model/sdm.py:245-277): tokenize with context 22, zero-pad to 77."""
     try:
         import clip  # third party: git+https://github.com/openai/CLIP.git (reference README.md:27)
@@ -321,6 +324,10 @@ def _default_clip_encoder(clip_version, device):
                            "or set model.text_encoder") from e
     clip_model, _ = clip.load(clip_version, device=device, jit=False)
     clip_model.eval()
+    if kernels:
+        from ..text import use_kernels
+        use_kernels(clip_model.transformer)
+        use_kernels(clip_model.ln_final)
 
     def encode(texts):
         tok = clip.tokenize(texts, context_length=22, truncate=True).to(device)
@@ -331,7 +338,7 @@ def _default_clip_encoder(clip_version, device):
     return encode
 
 
-def _default_bert_encoder(device):
+def _default_bert_encoder(device, kernels=False):
     """The reference's other text tower (model/sdm.py:261-264, 279-285): ``bert-base-uncased`` tokenizer with padding, the model's
     ``pooler_output`` (B,768) -- so the model must be built with ``clip_dim=768``.  Third party (``transformers`` + downloaded weights):
     parity unpinned, like CLIP; everything downstream of the (B,768) feature is pinned (golden G13)."""
@@ -343,6 +350,9 @@ def _default_bert_encoder(device):
         raise RuntimeError("the BERT text encoder is not available (%s): pass precomputed (B,768) text features as `y` or set "
                            "model.text_encoder" % type(e).__name__) from e
     bert.eval()
+    if kernels:
+        from ..text import use_kernels
+        use_kernels(bert)
     for p in bert.parameters():
         p.requires_grad = False
 
