@@ -13,45 +13,72 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 enum OpAct { OP_NONE = 0, OP_RELU, OP_GELU, OP_QUICK_GELU, OP_SILU, OP_SIGMOID, OP_TANH, OP_ACT_COUNT };
 
-template <class T> struct Half8;                                   // 8 elements of a 16-bit type as one 16-byte piece
-template <> struct Half8<__bf16> { typedef bfrag type; };
-template <> struct Half8<_Float16> { typedef hfrag type; };
+// Eight consecutive elements of a row as one memory access.  Rows of any width start anywhere, so the pieces are typed with the element's alignment:
+// gfx950 takes 16-byte global accesses at any address (the compiler emits one instruction), and an odd width costs a misaligned line per wave
+// instead of eight single-element accesses per piece.
+template <class T> struct Piece;
+template <> struct Piece<__bf16> { typedef bfrag frag; typedef bfrag mem __attribute__((aligned(2))); };
+template <> struct Piece<_Float16> { typedef hfrag frag; typedef hfrag mem __attribute__((aligned(2))); };
+template <> struct Piece<float> { typedef f32x4 frag; typedef f32x4 mem __attribute__((aligned(4))); };
+typedef u32x2 codes8 __attribute__((aligned(1)));
+typedef u32x4 codes16 __attribute__((aligned(1)));
 
-// ---- eight consecutive elements of a row <-> fp32 (the row piece is 16-byte aligned, 32 bytes long in fp32) ----
 template <class T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    const typename Half8<T>::type r = *reinterpret_cast<const typename Half8<T>::type*>(p);
+    typedef typename Piece<T>::mem mem;
+    if constexpr (sizeof(T) == 2) {
+        const typename Piece<T>::frag r = *reinterpret_cast<const mem*>(p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+        for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
+    } else {
+        const f32x4 a = *reinterpret_cast<const mem*>(p), b = *reinterpret_cast<const mem*>(p + 4);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+        for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    }
 }
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-    typename Half8<T>::type r;
+    typedef typename Piece<T>::mem mem;
+    if constexpr (sizeof(T) == 2) {
+        typename Piece<T>::frag r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
-    *reinterpret_cast<typename Half8<T>::type*>(p) = r;
+        for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
+        *reinterpret_cast<mem*>(p) = r;
+    } else {
+        *reinterpret_cast<mem*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<mem*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    }
 }
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
-    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-}
-// the same for a piece that may be unaligned or cut short: n valid elements (the others read as 0 / are not written)
+// a piece cut short by the row's end: n valid elements (n <= 0: none); the others read as 0 and are not written
 template <class T>
 __device__ __forceinline__ void load8n(const T* p, int n, float (&v)[8]) {
+    if (n >= 8) return load8(p, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
 }
 template <class T>
 __device__ __forceinline__ void store8n(T* p, int n, const float (&v)[8]) {
+    if (n >= 8) return store8(p, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) if (j < n) p[j] = (T)v[j];
+}
+// eight bytes (codes), the same way
+__device__ __forceinline__ u32x2 load_codes(const void* q, int n) {
+    const unsigned char* p = static_cast<const unsigned char*>(q);
+    if (n >= 8) return *reinterpret_cast<const codes8*>(p);
+    u32x2 w = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) w[j >> 2] |= (unsigned)p[j] << (8 * (j & 3));
+    return w;
+}
+__device__ __forceinline__ void store_codes(void* q, int n, const unsigned (&c)[8]) {
+    unsigned char* p = static_cast<unsigned char*>(q);
+    if (n >= 8) {
+        *reinterpret_cast<codes8*>(p) = u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) p[j] = (unsigned char)c[j];
 }
 // a parameter vector (bias, norm weight) is of the operand's type or fp32
 template <class T>
@@ -152,7 +179,6 @@ struct Epilogue {
     void* out = nullptr; long long ldo = 0;
     void* deriv = nullptr; long long ldd = 0; int form = DERIV_NONE;   // a'(z) for the backward pass
     int act = OP_NONE;
-    int vec = 0;                                                    // every row piece of 8 outputs is whole and 16-byte aligned
 };
 struct GemmArgs {
     const void *A = nullptr, *B = nullptr;                          // C(m, n) = sum_k A(m, k) B(n, k)

@@ -156,7 +156,6 @@ Bwd backward_layout(int dtype, int64_t M, int64_t N, int64_t K, bool dx, bool dw
 PrepJob padded(int dtype, const void* src, int64_t lds, int64_t rows, int64_t n, void* dst, int64_t ldd) {
     PrepJob j;
     j.src = src; j.lds = lds; j.dst = dst; j.ldd = ldd; j.rows = rows; j.n = (int)n; j.chunks = prep_chunks(rows, ldd);
-    j.vec_src = rows16(src, lds, 8, esize(dtype));
     return j;
 }
 int deriv_form(int dtype, int flags) { return flags & LSDM_OP_DERIV8 ? DERIV_8 : dtype == LSDM_F32 ? DERIV_F32 : DERIV_16; }
@@ -168,11 +167,12 @@ int check_linear(int dtype, int64_t M, int64_t N, int64_t K) {
     return LSDM_OK;
 }
 
-int norm_grid(int64_t rows, int D, bool vec, bool backward) {
-    const int rpg = norm_rows_per_group(D, vec);
-    const int64_t need = (rows + rpg - 1) / rpg;
-    // every work-group loads the parameters once; the backward pass also leaves one partial row each: as many as are resident, no more
-    const int64_t cap = backward ? 2 * kCUs : 8 * kCUs;
+// Work-groups of the norm kernels.  Each loads the parameters once, and in the backward pass leaves one partial row of dw and db: enough threads on a
+// CU to keep HBM busy, no more (backward, 32768 x 2048: bf16 1024 threads per CU 95 us, 512 of them 145 us, 1536 of them 101 us; fp32 512 of them
+// 148 us, 1024 of them 157 us; forward 2048 and 4096 of them the same).
+int norm_grid(int64_t rows, int D, bool backward, int es) {
+    const int threads = norm_threads(D), rpg = norm_rows_per_group(D);
+    const int64_t need = (rows + rpg - 1) / rpg, per_cu = (backward ? (es == 4 ? 512 : 1024) : 2048) / threads, cap = kCUs * (per_cu > 1 ? per_cu : 1);
     return (int)(need < cap ? need : cap);
 }
 
@@ -212,9 +212,8 @@ int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int
     e.out = y; e.ldo = N;
     e.act = activation;
     if (activation != LSDM_ACT_NONE && deriv) { e.deriv = deriv; e.ldd = N; e.form = deriv_form(dtype, flags); }
-    e.vec = N % 8 == 0 && aligned16(y) && (!e.res || rows16(residual, ldr, N, es)) && (!e.deriv || aligned16(deriv));
     if (f.rows) {
-        launch_rows(dtype, g, x_ok && w_ok, st);
+        launch_rows(dtype, g, st);
         return launched("lsdm_linear");
     }
     const int64_t kp = up(K, 8);
@@ -256,13 +255,11 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
         j.rows = M; j.n = (int)N; j.chunks = b.chunks;
         if (b.dz) { j.dst = b.z; j.ldd = b.ldz; z = b.z; ldz = b.ldz; }
         j.part = b.cs;
-        j.vec_src = rows16(dy, lddy, 8, es);
-        j.vec_deriv = aligned16(deriv) && N % 8 == 0;
     }
     if (b.xpad) {
         PrepJob& j = prep.job[jobs++];
         j = padded(dtype, codes ? codes : x, codes ? K : ldx, M, K, b.x, b.kp);
-        if (codes) { j.exps = static_cast<const unsigned char*>(exps); j.vec_src = K % 8 == 0 && ((uintptr_t)codes & 7) == 0; }
+        if (codes) j.exps = static_cast<const unsigned char*>(exps);
         xs = b.x; ldxs = b.kp;
     }
     if (b.wpad) { prep.job[jobs++] = padded(dtype, w, ldw, N, K, b.w, b.kp); ws_ = b.w; ldws = b.kp; }
@@ -278,7 +275,7 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
         g.M = (int)M; g.N = (int)K; g.K = (int)N;
         g.A = z; g.lda = ldz; g.B = ws_; g.ldb = ldws;
         g.part = b.partx;
-        g.e.out = dx; g.e.ldo = K; g.e.vec = K % 8 == 0 && aligned16(dx);
+        g.e.out = dx; g.e.ldo = K;
         launch_gemm(dtype, b.px, g, KM, st);
     }
     if (dw) {
@@ -286,7 +283,7 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
         g.M = (int)N; g.N = (int)K; g.K = (int)M;
         g.A = z; g.lda = ldz; g.B = xs; g.ldb = ldxs;
         g.part = b.partw;
-        g.e.out = dw; g.e.ldo = K; g.e.vec = K % 8 == 0 && aligned16(dw);
+        g.e.out = dw; g.e.ldo = K;
         launch_gemm(dtype, b.pw, g, MM, st);
     }
     return launched("lsdm_linear_backward");
@@ -294,9 +291,7 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
 
 int64_t lsdm_layer_norm_workspace(int64_t rows, int64_t D) {
     if (rows < 1 || D < 1 || D > kNormMaxWidth) return refuse(LSDM_ERR_ARG, "lsdm_layer_norm: rows >= 1 and a width in [1, %d] are needed", kNormMaxWidth);
-    // (either variant's grid; the larger one)
-    const int64_t g1 = norm_grid(rows, (int)D, true, true), g2 = norm_grid(rows, (int)D, false, true);
-    return (g1 > g2 ? g1 : g2) * 2 * D * 4;
+    return (int64_t)norm_grid(rows, (int)D, true, 2) * 2 * D * 4;      // (16-bit calls have the larger grid)
 }
 
 static int check_norm(const char* who, int dtype, int64_t rows, int64_t D) {
@@ -316,9 +311,7 @@ int lsdm_layer_norm(int device, int dtype, int flags, int64_t rows, int64_t D, c
     NormArgs a;
     a.rows = rows; a.D = (int)D; a.eps = eps; a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.param_f32 = flags & LSDM_OP_PARAM_F32 ? 1 : 0;
     a.y = y; a.mean = mean; a.rstd = rstd; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps;
-    const int es = esize(dtype);
-    const bool vec = D % 8 == 0 && rows16(x, ldx, D, es) && aligned16(y) && aligned16(codes);
-    launch_norm(dtype, a, vec, norm_grid(rows, (int)D, vec, false), false, static_cast<hipStream_t>(stream));
+    launch_norm(dtype, a, norm_grid(rows, (int)D, false, esize(dtype)), false, static_cast<hipStream_t>(stream));
     return launched("lsdm_layer_norm");
 }
 
@@ -339,10 +332,8 @@ int lsdm_layer_norm_backward(int device, int dtype, int flags, int64_t rows, int
     a.rows = rows; a.D = (int)D; a.x = codes ? nullptr : x; a.ldx = ldx; a.w = w; a.param_f32 = flags & LSDM_OP_PARAM_F32 ? 1 : 0;
     a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.codes = (signed char*)codes; a.exps = (unsigned char*)exps;
     a.dy = dy; a.lddy = lddy; a.dx = dx; a.part = part ? static_cast<float*>(ws) : nullptr;
-    const int es = esize(dtype);
-    const bool vec = D % 8 == 0 && rows16(dy, lddy, D, es) && (codes ? aligned16(codes) : rows16(x, ldx, D, es)) && (!dx || aligned16(dx));
-    const int grid = norm_grid(rows, (int)D, vec, true);
-    launch_norm(dtype, a, vec, grid, true, st);
+    const int grid = norm_grid(rows, (int)D, true, esize(dtype));
+    launch_norm(dtype, a, grid, true, st);
     if (part) launch_norm_join(dtype, a.part, grid, (int)D, dw, db, a.param_f32, st);
     return launched("lsdm_layer_norm_backward");
 }
@@ -353,7 +344,7 @@ int lsdm_pack8(int device, int dtype, int64_t rows, int64_t D, const void* x, in
     if (!dev.ok) return LSDM_ERR_HIP;
     Pack8Args a;
     a.rows = rows; a.D = (int)D; a.x = x; a.ldx = ldx; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps;
-    launch_pack8(dtype, a, D % 32 == 0 && rows16(x, ldx, D, esize(dtype)) && aligned16(codes), static_cast<hipStream_t>(stream));
+    launch_pack8(dtype, a, static_cast<hipStream_t>(stream));
     return launched("lsdm_pack8");
 }
 
@@ -363,7 +354,7 @@ int lsdm_unpack8(int device, int dtype, int64_t rows, int64_t D, const void* cod
     if (!dev.ok) return LSDM_ERR_HIP;
     Pack8Args a;
     a.rows = rows; a.D = (int)D; a.codes = (signed char*)codes; a.exps = (unsigned char*)exps; a.out = out;
-    launch_unpack8(dtype, a, D % 32 == 0 && aligned16(out) && aligned16(codes), static_cast<hipStream_t>(stream));
+    launch_unpack8(dtype, a, static_cast<hipStream_t>(stream));
     return launched("lsdm_unpack8");
 }
 

@@ -170,7 +170,7 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
     float y[8], d[8], r[8];
     if (e.res) {
         const T* p = static_cast<const T*>(e.res) + m * e.ldr + n;
-        if (e.vec) load8(p, r); else load8n(p, cnt, r);
+        load8n(p, cnt, r);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) z[j] += bias[j];
@@ -182,28 +182,26 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
         for (int j = 0; j < 8; ++j) act_eval<T>(e.act, z[j], want, y[j], d[j]);
         if (want) {
             if (e.form == DERIV_8) {
-                unsigned char* p = static_cast<unsigned char*>(e.deriv) + m * e.ldd + n;
                 unsigned c[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) c[j] = deriv_code8(d[j]);
-                if (e.vec) *reinterpret_cast<u32x2*>(p) = u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
-                else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) if (j < cnt) p[j] = (unsigned char)c[j];
-                }
+                store_codes(static_cast<unsigned char*>(e.deriv) + m * e.ldd + n, cnt, c);
             } else if constexpr (sizeof(T) == 2) {
-                unsigned short* p = static_cast<unsigned short*>(e.deriv) + m * e.ldd + n;
-                unsigned c[8];
+                T v[8];                          // (the 16-bit form travels as T's bits)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) c[j] = deriv_code16(d[j]);
-                if (e.vec) *reinterpret_cast<u32x4*>(p) = u32x4{c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16};
-                else {
+                for (int j = 0; j < 8; ++j) v[j] = __builtin_bit_cast(T, (unsigned short)deriv_code16(d[j]));
+                T* p = static_cast<T*>(e.deriv) + m * e.ldd + n;
+                if (cnt >= 8) {
+                    typename Piece<T>::frag f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) if (j < cnt) p[j] = (unsigned short)c[j];
+                    for (int j = 0; j < 8; ++j) f[j] = v[j];
+                    *reinterpret_cast<typename Piece<T>::mem*>(p) = f;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) if (j < cnt) p[j] = v[j];
                 }
             } else {
-                float* p = static_cast<float*>(e.deriv) + m * e.ldd + n;
-                if (e.vec) store8(p, d); else store8n(p, cnt, d);
+                store8n(static_cast<float*>(e.deriv) + m * e.ldd + n, cnt, d);
             }
         }
     }
@@ -212,7 +210,7 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
         for (int j = 0; j < 8; ++j) y[j] += r[j];
     }
     T* p = static_cast<T*>(e.out) + m * e.ldo + n;
-    if (e.vec) store8(p, y); else store8n(p, cnt, y);
+    store8n(p, cnt, y);
 }
 template <class T>
 __device__ __forceinline__ void bias8(const Epilogue& e, int n, int N, float (&b)[8]) {
@@ -358,12 +356,14 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
         for (int r = 0; r < RW; r += RPI) {
             const int m = em + r;
             float z[8];
-            load8(reinterpret_cast<const float*>(mine + (r + lane / CPR) * PITCH + (lane % CPR) * 32), z);
+            const f32x4* zp = reinterpret_cast<const f32x4*>(mine + (r + lane / CPR) * PITCH + (lane % CPR) * 32);
+            const f32x4 z0 = zp[0], z1 = zp[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { z[j] = z0[j]; z[4 + j] = z1[j]; }
             if (m < g.M) {
                 if (g.splits > 1) {
                     float* p = g.part + ((long long)ks * g.M + m) * g.N + en;
-                    if ((g.N & 7) == 0) { if (en < g.N) store8(p, z); }
-                    else store8n(p, g.N - en, z);
+                    store8n(p, g.N - en, z);
                 } else {
                     epilogue8<T>(g.e, z, bias, m, en, g.N);
                 }
@@ -384,41 +384,25 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g, long long pieces,
     bias8<T>(g.e, n, g.N, bias);
     const long long slab = (long long)g.M * g.N;
     const float* p = g.part + m * g.N + n;
-    if ((g.N & 7) == 0) {
 #pragma unroll 4
-        for (int s = 0; s < g.splits; ++s) {
-            float v[8];
-            load8(p + s * slab, v);
+    for (int s = 0; s < g.splits; ++s) {
+        float v[8];
+        load8n(p + s * slab, g.N - n, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] += v[j];
-        }
-    } else {
-        for (int s = 0; s < g.splits; ++s) {
-            float v[8];
-            load8n(p + s * slab, g.N - n, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] += v[j];
-        }
+        for (int j = 0; j < 8; ++j) z[j] += v[j];
     }
     epilogue8<T>(g.e, z, bias, m, n, g.N);
 }
 
 // ---- few rows: M <= 16 MB.  A work-group owns 16 columns; its waves split k and join through LDS.  W is read once, straight into fragments;
-// any K and any alignment (the fragment loads fall back to single elements). ----
-template <class T, bool ALIGNED>
+// any K and any alignment. ----
+template <class T>
 __device__ __forceinline__ typename Mma<T>::frag row_frag(const T* p, int k, int K) {
     typename Mma<T>::frag f;
     constexpr int E = sizeof(T) == 4 ? 4 : 8;
-    if constexpr (ALIGNED) {
-        if (k < K) f = *reinterpret_cast<const typename Mma<T>::frag*>(p + k);
-        else {
+    if (k + E <= K) return *reinterpret_cast<const typename Piece<T>::mem*>(p + k);
 #pragma unroll
-            for (int j = 0; j < E; ++j) f[j] = (T)0.0f;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) f[j] = k + j < K ? p[k + j] : (T)0.0f;
-    }
+    for (int j = 0; j < E; ++j) f[j] = k + j < K ? p[k + j] : (T)0.0f;
     return f;
 }
 template <class T> struct RowMma {
@@ -431,7 +415,7 @@ template <> struct RowMma<float> {
         return c;
     }
 };
-template <class T, int MB, bool ALIGNED>
+template <class T, int MB>
 __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs g) {
     constexpr int E = sizeof(T) == 4 ? 4 : 8, KSTEP = 4 * E;        // k of one instruction group over the four 16-lane groups
     __shared__ float part[MB == 4 ? 8 : 16][MB * 16][16 + 4];        // (one slab per wave: launch_rows_t starts at most that many)
@@ -452,9 +436,9 @@ __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs g) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (s0 + u * nw) * KSTEP + kl;
-            fw[u] = row_frag<T, ALIGNED>(w, k, g.K);
+            fw[u] = row_frag<T>(w, k, g.K);
 #pragma unroll
-            for (int b = 0; b < MB; ++b) fx[u][b] = row_frag<T, ALIGNED>(x[b], k, g.K);
+            for (int b = 0; b < MB; ++b) fx[u][b] = row_frag<T>(x[b], k, g.K);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -499,43 +483,30 @@ __global__ __launch_bounds__(256) void prep_kernel(PrepArgs args) {
             if (a.exps) {
                 const signed char* q = static_cast<const signed char*>(a.src) + r * a.n + c0;
                 const float step = n > 0 ? exp8_step(a.exps[r * gpr + (c0 >> 5)]) : 0.0f;
-                if (a.vec_src && n == 8) {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(q);
+                const u32x2 w = load_codes(q, n);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = (float)((int)(w[j >> 2] << (24 - 8 * (j & 3))) >> 24) * step;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)q[j] * step : 0.0f;
-                }
+                for (int j = 0; j < 8; ++j) v[j] = (float)((int)(w[j >> 2] << (24 - 8 * (j & 3))) >> 24) * step;
             } else {
-                const T* p = static_cast<const T*>(a.src) + r * a.lds + c0;
-                if (a.vec_src && n == 8) load8(p, v); else load8n(p, n, v);
+                load8n(static_cast<const T*>(a.src) + r * a.lds + c0, n, v);
             }
             if (a.form != DERIV_NONE) {
                 const long long at = r * a.n + c0;
                 if (a.form == DERIV_8) {
-                    const unsigned char* q = static_cast<const unsigned char*>(a.deriv) + at;
-                    if (a.vec_deriv) {
-                        const u32x2 w = *reinterpret_cast<const u32x2*>(q);
+                    const u32x2 w = load_codes(static_cast<const unsigned char*>(a.deriv) + at, n);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] = deriv_value8((w[j >> 2] >> (8 * (j & 3))) & 255u);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value8(q[j]) : 0.0f;
-                    }
+                    for (int j = 0; j < 8; ++j) d[j] = deriv_value8((w[j >> 2] >> (8 * (j & 3))) & 255u);
                 } else if constexpr (sizeof(T) == 2) {
-                    const unsigned short* q = static_cast<const unsigned short*>(a.deriv) + at;
-                    if (a.vec_deriv) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(q);
+                    const T* q = static_cast<const T*>(a.deriv) + at;
+                    if (n >= 8) {
+                        const typename Piece<T>::frag f = *reinterpret_cast<const typename Piece<T>::mem*>(q);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] = deriv_value16((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+                        for (int j = 0; j < 8; ++j) d[j] = deriv_value16(__builtin_bit_cast(unsigned short, (T)f[j]));
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value16(q[j]) : 0.0f;
+                        for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value16(__builtin_bit_cast(unsigned short, q[j])) : 0.0f;
                     }
                 } else {
-                    const float* q = static_cast<const float*>(a.deriv) + at;
-                    if (a.vec_deriv) load8(q, d); else load8n(q, n, d);
+                    load8n(static_cast<const float*>(a.deriv) + at, n, d);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] * d[j] : 0.0f;
@@ -589,7 +560,7 @@ void launch_gemm_t(const GemmPlan& p, GemmArgs g, int layout, hipStream_t st) {
 }
 
 template <class T>
-void launch_rows_t(const GemmArgs& g, bool aligned, hipStream_t st) {
+void launch_rows_t(const GemmArgs& g, hipStream_t st) {
     const dim3 grid((unsigned)((g.N + 15) / 16));
     constexpr int KSTEP = sizeof(T) == 4 ? 16 : 32;
     const int steps = (g.K + KSTEP - 1) / KSTEP;
@@ -602,8 +573,7 @@ void launch_rows_t(const GemmArgs& g, bool aligned, hipStream_t st) {
         constexpr int MB = decltype(mb)::value;
         // the join needs 32 MB threads
         const dim3 bb(b.x < 32 * MB ? 32 * MB : b.x);
-        if (aligned) hipLaunchKernelGGL((rows_kernel<T, MB, true>), grid, bb, 0, st, g);
-        else hipLaunchKernelGGL((rows_kernel<T, MB, false>), grid, bb, 0, st, g);
+        hipLaunchKernelGGL((rows_kernel<T, MB>), grid, bb, 0, st, g);
     };
     if (g.M <= 16) go(std::integral_constant<int, 1>{});
     else if (g.M <= 32) go(std::integral_constant<int, 2>{});
@@ -615,10 +585,10 @@ void launch_gemm(int dtype, const GemmPlan& p, const GemmArgs& g, int layout, hi
     else if (dtype == 1) launch_gemm_t<__bf16>(p, g, layout, st);
     else launch_gemm_t<_Float16>(p, g, layout, st);
 }
-void launch_rows(int dtype, const GemmArgs& g, bool aligned, hipStream_t st) {
-    if (dtype == 0) launch_rows_t<float>(g, aligned, st);
-    else if (dtype == 1) launch_rows_t<__bf16>(g, aligned, st);
-    else launch_rows_t<_Float16>(g, aligned, st);
+void launch_rows(int dtype, const GemmArgs& g, hipStream_t st) {
+    if (dtype == 0) launch_rows_t<float>(g, st);
+    else if (dtype == 1) launch_rows_t<__bf16>(g, st);
+    else launch_rows_t<_Float16>(g, st);
 }
 void launch_prep(int dtype, const PrepArgs& a, int jobs, hipStream_t st) {
     unsigned x = 1, y = 1;

@@ -18,7 +18,6 @@ struct PrepJob {
     void* dst = nullptr; long long ldd = 0;          // NULL: only the column sums; ldd a multiple of 8 elements, rows 16-byte aligned
     float* part = nullptr;                           // (chunks, n) column sums, or NULL
     long long rows = 0; int n = 0, chunks = 1;
-    int vec_src = 0, vec_deriv = 0;                  // whole 8-element pieces may be read with vector loads (vec_deriv: all of them are whole)
 };
 struct PrepArgs { PrepJob job[3]; };
 
@@ -41,14 +40,15 @@ struct Pack8Args {
 };
 
 void launch_gemm(int dtype, const GemmPlan& p, const GemmArgs& g, int layout, hipStream_t st);
-void launch_rows(int dtype, const GemmArgs& g, bool aligned, hipStream_t st);
+void launch_rows(int dtype, const GemmArgs& g, hipStream_t st);
 void launch_prep(int dtype, const PrepArgs& a, int jobs, hipStream_t st);
 void launch_colsum_join(int dtype, const GemmArgs& g, hipStream_t st);
-void launch_norm(int dtype, const NormArgs& a, bool vec, int grid, bool backward, hipStream_t st);
+void launch_norm(int dtype, const NormArgs& a, int grid, bool backward, hipStream_t st);
 void launch_norm_join(int dtype, const float* part, int groups, int D, void* dw, void* db, int param_f32, hipStream_t st);
-int norm_rows_per_group(int D, bool vec);            // rows a work-group of the norm kernels has in flight
-void launch_pack8(int dtype, const Pack8Args& a, bool wide, hipStream_t st);
-void launch_unpack8(int dtype, const Pack8Args& a, bool wide, hipStream_t st);
+int norm_threads(int D);                             // threads of a work-group of the norm kernels, and the rows it has in flight
+int norm_rows_per_group(int D);
+void launch_pack8(int dtype, const Pack8Args& a, hipStream_t st);
+void launch_unpack8(int dtype, const Pack8Args& a, hipStream_t st);
 
 }  // namespace ops
 }  // namespace lsdm

@@ -8,142 +8,168 @@
 // threads for rows of up to 64 columns up to 1024 threads for 16384, so that a lane holds 8 or 16 values.  A work-group walks many rows: the
 // parameters stay in registers, and the backward pass adds dw / db per lane over its rows and writes ONE partial row per work-group, joined in
 // order by a second launch (no atomics: results do not depend on the schedule).
-// VEC: 16-byte pieces (a lane's columns are (lane + NT i) 8 + j); otherwise -- odd widths, unaligned rows -- single elements, lane-interleaved
-// (column (8 i + j) NT + lane), which stays coalesced.
+// A row is read and written in pieces of eight elements (ops.hpp), whatever its width and alignment.
 #include "ops.hpp"
 #include "ops_launch.hpp"
 
 namespace lsdm {
 namespace ops {
 
+// Sum / maximum over groups of W = 4 .. 64 neighbouring lanes, the result in all of them: within 16 lanes by DPP operands of the addition itself (quad
+// permutes, then the mirrored half and full rows), across rows by the 16- and 32-lane swaps.  No LDS round trips (__shfl_xor is one per level).
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <int W, class F>
+__device__ __forceinline__ unsigned lanes_join(unsigned v, F f) {
+    if constexpr (W >= 2) v = f(v, dpp<0xB1>(v));            // lanes 1 0 3 2
+    if constexpr (W >= 4) v = f(v, dpp<0x4E>(v));            // lanes 2 3 0 1
+    if constexpr (W >= 8) v = f(v, dpp<0x141>(v));           // mirrored within 8
+    if constexpr (W >= 16) v = f(v, dpp<0x140>(v));          // mirrored within 16
+    if constexpr (W >= 32) { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); v = f(r[0], r[1]); }
+    if constexpr (W >= 64) { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); v = f(r[0], r[1]); }
+    return v;
+}
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return __builtin_bit_cast(float, lanes_join<W>(__builtin_bit_cast(unsigned, v), [](unsigned a, unsigned b) {
+        return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }));
+}
+template <int W>
+__device__ __forceinline__ unsigned lanes_max(unsigned v) { return lanes_join<W>(v, [](unsigned a, unsigned b) { return max(a, b); }); }
+
+// both sums over the NT threads of a row; red: one entry per wave of the work-group
 template <int NT>
 __device__ __forceinline__ float2 row_sum2(float a, float b, float2* red, int t) {
-    constexpr int W = NT < 64 ? NT : 64;
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+    a = lanes_sum<(NT < 64 ? NT : 64)>(a);
+    b = lanes_sum<(NT < 64 ? NT : 64)>(b);
     if constexpr (NT > 64) {
         constexpr int NW = NT / 64;
+        const int first = (t / NT) * NW;         // the row's waves
         wg_sync();                               // (the previous sums have been read)
         if ((t & 63) == 0) red[t >> 6] = make_float2(a, b);
         wg_sync();
         a = 0.0f; b = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) { a += red[i].x; b += red[i].y; }
+        for (int i = 0; i < NW; ++i) { a += red[first + i].x; b += red[first + i].y; }
     }
     return make_float2(a, b);
 }
 
-template <int NT, bool VEC>
-__device__ __forceinline__ int col_of(int l, int i, int j) { return VEC ? (l + NT * i) * 8 + j : (i * 8 + j) * NT + l; }
+// lane l of a row's NT threads holds the pieces of 8 columns l, l + NT, ...  WHOLE: the width is a multiple of 8, so a piece is valid or not as one.
+template <int NT>
+__device__ __forceinline__ int col_of(int l, int i) { return (l + NT * i) * 8; }
 
-template <class T, int NT, int NV, bool VEC>
-__device__ __forceinline__ void row_load(const T* p, int D, int l, float (&v)[NV][8]) {
+// p: a row that exists (of D elements); n: D, or 0 where the values are not wanted.  The loads stand in no branch -- a lane without a whole piece reads
+// the row's first one and drops it -- so that all of a row's are in flight together; only the piece cut short by the row's end takes a branch.
+template <class T, int NT, int NV, bool WHOLE>
+__device__ __forceinline__ void row_load(const T* p, int D, int n, int l, float (&v)[NV][8]) {
+    typedef typename Piece<T>::frag frag;
+    typedef typename Piece<T>::mem mem;
+    constexpr int H = 8 * (int)sizeof(T) / 16;
+    frag raw[NV][H];
+    if (WHOLE || D >= 8) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = col_of<NT>(l, i), at = c + 8 <= n ? c : 0;
+#pragma unroll
+            for (int k = 0; k < H; ++k) raw[i][k] = *reinterpret_cast<const mem*>(p + at + k * (8 / H));
+        }
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if constexpr (VEC) {
-            if ((l + NT * i) * 8 < D) load8(p + (l + NT * i) * 8, v[i]);
-            else {
+        const bool full = col_of<NT>(l, i) + 8 <= n;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        for (int j = 0; j < 8; ++j) v[i][j] = full ? (float)raw[i][j / (8 / H)][j % (8 / H)] : 0.0f;
+    }
+    if constexpr (!WHOLE) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = col_of<NT>(l, i);
+            if (c < n && c + 8 > n) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (j < n - c) v[i][j] = (float)p[c + j];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { const int c = col_of<NT, VEC>(l, i, j); v[i][j] = c < D ? (float)p[c] : 0.0f; }
         }
     }
 }
-template <class T, int NT, int NV, bool VEC>
+template <class T, int NT, int NV, bool WHOLE>
 __device__ __forceinline__ void row_store(T* p, int D, int l, const float (&v)[NV][8]) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if constexpr (VEC) {
-            if ((l + NT * i) * 8 < D) store8(p + (l + NT * i) * 8, v[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { const int c = col_of<NT, VEC>(l, i, j); if (c < D) p[c] = (T)v[i][j]; }
+        const int c = col_of<NT>(l, i);
+        if (c < D) {
+            if constexpr (WHOLE) store8(p + c, v[i]); else store8n(p + c, D - c, v[i]);
         }
     }
 }
 
-// the row's 8-bit checkpoint: groups of 32 columns are four lanes' pieces (VEC) or 32 lanes' single elements
-template <int NT, int NV, bool VEC>
+// the row's 8-bit checkpoint: a group of 32 columns is four lanes' pieces
+template <int NT, int NV, bool WHOLE>
 __device__ __forceinline__ void row_encode(const float (&h)[NV][8], int D, int l, signed char* codes, unsigned char* exps) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if constexpr (VEC) {
-            unsigned m = 0;
+        unsigned m = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __builtin_bit_cast(unsigned, h[i][j]) & 0x7fffffffu);   // (order of the bit patterns: NaN is largest)
-            m = max(m, (unsigned)__shfl_xor((int)m, 1));
-            m = max(m, (unsigned)__shfl_xor((int)m, 2));
-            const unsigned b = exp8_of_amax(__builtin_bit_cast(float, m));
-            const float inv = exp8_inv(b);
-            const int c = (l + NT * i) * 8;
-            if (c < D) {
-                unsigned q[8];
+        for (int j = 0; j < 8; ++j) m = max(m, __builtin_bit_cast(unsigned, h[i][j]) & 0x7fffffffu);   // (order of the bit patterns: NaN is largest)
+        const unsigned b = exp8_of_amax(__builtin_bit_cast(float, lanes_max<4>(m)));
+        const float inv = exp8_inv(b);
+        const int c = col_of<NT>(l, i);
+        if (c < D) {
+            unsigned q[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = (unsigned)code8(h[i][j], inv) & 255u;
-                *reinterpret_cast<u32x2*>(codes + c) = u32x2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
-                if ((l & 3) == 0) exps[c >> 5] = (unsigned char)b;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = col_of<NT, VEC>(l, i, j);
-                unsigned m = c < D ? __builtin_bit_cast(unsigned, h[i][j]) & 0x7fffffffu : 0u;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
-                const unsigned b = exp8_of_amax(__builtin_bit_cast(float, m));
-                if (c < D) {
-                    codes[c] = (signed char)code8(h[i][j], exp8_inv(b));
-                    if ((l & 31) == 0) exps[c >> 5] = (unsigned char)b;
-                }
-            }
+            for (int j = 0; j < 8; ++j) q[j] = (unsigned)code8(h[i][j], inv) & 255u;
+            store_codes(codes + c, WHOLE ? 8 : D - c, q);
+            if ((l & 3) == 0) exps[c >> 5] = (unsigned char)b;
         }
     }
 }
-template <int NT, int NV, bool VEC>
-__device__ __forceinline__ void row_decode(const signed char* codes, const unsigned char* exps, int D, int l, float (&h)[NV][8]) {
+template <int NT, int NV, bool WHOLE>
+__device__ __forceinline__ void row_decode(const signed char* codes, const unsigned char* exps, int D, int n, int l, float (&h)[NV][8]) {
+    u32x2 w[NV];
+    unsigned b[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if constexpr (VEC) {
-            const int c = (l + NT * i) * 8;
-            u32x2 w = {0, 0};
-            float s = 0.0f;
-            if (c < D) { w = *reinterpret_cast<const u32x2*>(codes + c); s = exp8_step(exps[c >> 5]); }
+        const int c = col_of<NT>(l, i);
+        b[i] = exps[c < n ? c >> 5 : 0];
+        if (WHOLE || D >= 8) w[i] = *reinterpret_cast<const codes8*>(codes + (c + 8 <= n ? c : 0));
+        if constexpr (!WHOLE) { if (c < n && c + 8 > n) w[i] = load_codes(codes + c, n - c); }
+    }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = (float)((int)(w[j >> 2] << (24 - 8 * (j & 3))) >> 24) * s;
-        } else {
+    for (int i = 0; i < NV; ++i) {
+        const bool any = col_of<NT>(l, i) < n;
+        const float s = exp8_step(b[i]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = col_of<NT, VEC>(l, i, j);
-                h[i][j] = c < D ? (float)codes[c] * exp8_step(exps[c >> 5]) : 0.0f;
-            }
-        }
+        for (int j = 0; j < 8; ++j) h[i][j] = any ? (float)((int)(w[i][j >> 2] << (24 - 8 * (j & 3))) >> 24) * s : 0.0f;
     }
 }
 
-template <class T, int NT, int NV, bool VEC>
+template <class T, int NT, int NV, bool WHOLE>
 __device__ __forceinline__ void param_load(const void* p, int is_f32, float missing, int D, int l, float (&v)[NV][8]) {
+    if (p && is_f32) return row_load<float, NT, NV, WHOLE>(static_cast<const float*>(p), D, D, l, v);
+    if (p) return row_load<T, NT, NV, WHOLE>(static_cast<const T*>(p), D, D, l, v);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { const int c = col_of<NT, VEC>(l, i, j); v[i][j] = p && c < D ? param<T>(p, is_f32, c) : (c < D ? missing : 0.0f); }
+        for (int j = 0; j < 8; ++j) v[i][j] = missing;
 }
 
-template <class T, int NT, int NV, bool VEC>
+template <class T, int NT, int NV, bool WHOLE>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_fwd_kernel(NormArgs a) {
     constexpr int THREADS = NT > 256 ? NT : 256, RPG = THREADS / NT;
-    __shared__ float2 red[NT > 64 ? NT / 64 : 1];
+    __shared__ float2 red[THREADS / 64];
     const int t = threadIdx.x, l = t % NT, D = a.D;
     float w[NV][8], b[NV][8];
-    param_load<T, NT, NV, VEC>(a.w, a.param_f32, 1.0f, D, l, w);
-    param_load<T, NT, NV, VEC>(a.b, a.param_f32, 0.0f, D, l, b);
+    param_load<T, NT, NV, WHOLE>(a.w, a.param_f32, 1.0f, D, l, w);
+    param_load<T, NT, NV, WHOLE>(a.b, a.param_f32, 0.0f, D, l, b);
     const float inv_d = 1.0f / (float)D;
-    // (a work-group of one row per NT <= 64 threads has no barrier: its rows end independently; with NT > 64 the loop is uniform)
-    for (long long r = (long long)blockIdx.x * RPG + t / NT; r < a.rows; r += (long long)gridDim.x * RPG) {
+    // (the loop is uniform over the work-group, as its barriers need it: a group of threads without a row left works on zeros and stores nothing)
+    for (long long r0 = (long long)blockIdx.x * RPG; r0 < a.rows; r0 += (long long)gridDim.x * RPG) {
+        const long long r = r0 + t / NT;
+        const bool live = r < a.rows;
+        const long long rr = live ? r : a.rows - 1;
         float x[NV][8];
-        row_load<T, NT, NV, VEC>(static_cast<const T*>(a.x) + r * a.ldx, D, l, x);
+        row_load<T, NT, NV, WHOLE>(static_cast<const T*>(a.x) + rr * a.ldx, D, live ? D : 0, l, x);
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -155,51 +181,59 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_fwd_kernel(NormArgs 
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { x[i][j] = col_of<NT, VEC>(l, i, j) < D ? x[i][j] - mu : 0.0f; s += x[i][j]; q = fmaf(x[i][j], x[i][j], q); }
+            for (int j = 0; j < 8; ++j) {
+                x[i][j] -= col_of<NT>(l, i) + (WHOLE ? 0 : j) < D ? mu : 0.0f;      // (columns beyond the row are 0 and stay 0)
+                s += x[i][j];
+                q = fmaf(x[i][j], x[i][j], q);
+            }
         const float2 c = row_sum2<NT>(s, q, red, t);
         const float d = c.x * inv_d, rstd = 1.0f / sqrtf(fmaxf(fmaf(c.y, inv_d, -d * d), 0.0f) + a.eps);
         mu += d;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[i][j] = col_of<NT, VEC>(l, i, j) < D ? (x[i][j] - d) * rstd : 0.0f;
-        if (a.mean && l == 0) a.mean[r] = mu;
-        if (a.rstd && l == 0) a.rstd[r] = rstd;
-        if (a.codes) row_encode<NT, NV, VEC>(x, D, l, a.codes + r * D, a.exps + r * ((D + 31) >> 5));
+            for (int j = 0; j < 8; ++j) x[i][j] = (x[i][j] - (col_of<NT>(l, i) + (WHOLE ? 0 : j) < D ? d : 0.0f)) * rstd;
+        if (a.mean && live && l == 0) a.mean[r] = mu;
+        if (a.rstd && live && l == 0) a.rstd[r] = rstd;
+        if (a.codes) row_encode<NT, NV, WHOLE>(x, live ? D : 0, l, a.codes + r * D, a.exps + r * ((D + 31) >> 5));
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[i][j] = fmaf(x[i][j], w[i][j], b[i][j]);
-        row_store<T, NT, NV, VEC>(static_cast<T*>(a.y) + r * D, D, l, x);
+        row_store<T, NT, NV, WHOLE>(static_cast<T*>(a.y) + r * D, live ? D : 0, l, x);
     }
 }
 
-template <class T, int NT, int NV, bool VEC>
+template <class T, int NT, int NV, bool WHOLE>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_bwd_kernel(NormArgs a) {
     constexpr int THREADS = NT > 256 ? NT : 256, RPG = THREADS / NT, COLS = NT * NV * 8;
-    __shared__ float2 red[NT > 64 ? NT / 64 : 1];
+    __shared__ float2 red[THREADS / 64];
     __shared__ float join[RPG > 1 ? RPG : 1][RPG > 1 ? COLS + 1 : 1];
     const int t = threadIdx.x, l = t % NT, D = a.D;
     float w[NV][8], dw[NV][8], db[NV][8];
-    param_load<T, NT, NV, VEC>(a.w, a.param_f32, 1.0f, D, l, w);
+    param_load<T, NT, NV, WHOLE>(a.w, a.param_f32, 1.0f, D, l, w);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.0f;
     const float inv_d = 1.0f / (float)D;
-    for (long long r = (long long)blockIdx.x * RPG + t / NT; r < a.rows; r += (long long)gridDim.x * RPG) {
+    for (long long r0 = (long long)blockIdx.x * RPG; r0 < a.rows; r0 += (long long)gridDim.x * RPG) {       // (uniform, as above)
+        const long long r = r0 + t / NT;
+        const bool live = r < a.rows;
+        const long long rr = live ? r : a.rows - 1;
+        const int n = live ? D : 0;
         float g[NV][8], h[NV][8];
-        row_load<T, NT, NV, VEC>(static_cast<const T*>(a.dy) + r * a.lddy, D, l, g);
-        const float rstd = a.rstd[r];
+        row_load<T, NT, NV, WHOLE>(static_cast<const T*>(a.dy) + rr * a.lddy, D, n, l, g);
+        const float rstd = a.rstd[rr];
         if (a.codes) {
-            row_decode<NT, NV, VEC>(a.codes + r * D, a.exps + r * ((D + 31) >> 5), D, l, h);
+            row_decode<NT, NV, WHOLE>(a.codes + rr * D, a.exps + rr * ((D + 31) >> 5), D, n, l, h);
         } else {
-            row_load<T, NT, NV, VEC>(static_cast<const T*>(a.x) + r * a.ldx, D, l, h);
-            const float mu = a.mean[r];
+            row_load<T, NT, NV, WHOLE>(static_cast<const T*>(a.x) + rr * a.ldx, D, n, l, h);
+            const float mu = a.mean[rr];
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] = col_of<NT, VEC>(l, i, j) < D ? (h[i][j] - mu) * rstd : 0.0f;
+                for (int j = 0; j < 8; ++j) h[i][j] = (h[i][j] - mu) * rstd;        // (columns beyond the row: g = 0 there, so h does not matter)
         }
         float s = 0.0f, q = 0.0f;
 #pragma unroll
@@ -219,7 +253,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_bwd_kernel(NormArgs 
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[i][j] = rstd * (g[i][j] - c1 - h[i][j] * c2);
-            row_store<T, NT, NV, VEC>(static_cast<T*>(a.dx) + r * D, D, l, g);
+            row_store<T, NT, NV, WHOLE>(static_cast<T*>(a.dx) + r * D, n, l, g);
         }
     }
     if (!a.part) return;
@@ -229,7 +263,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_bwd_kernel(NormArgs 
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { const int c = col_of<NT, VEC>(l, i, j); if (c < D) { out[c] = dw[i][j]; out[D + c] = db[i][j]; } }
+            for (int j = 0; j < 8; ++j) { const int c = col_of<NT>(l, i) + j; if (c < D) { out[c] = dw[i][j]; out[D + c] = db[i][j]; } }
     } else {
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -237,7 +271,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_bwd_kernel(NormArgs 
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) join[t / NT][col_of<NT, VEC>(l, i, j)] = which ? db[i][j] : dw[i][j];
+                for (int j = 0; j < 8; ++j) join[t / NT][col_of<NT>(l, i) + j] = which ? db[i][j] : dw[i][j];
             wg_sync();
             for (int c = t; c < D; c += THREADS) {
                 float v = 0.0f;
@@ -271,43 +305,40 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const float* __restrict_
 
 namespace {
 
-// threads per row and pieces per thread for a width: up to 1024 columns a row stays within one wave (no barrier), beyond that it is a work-group's
-template <class T, bool VEC, class F>
+// threads per row and pieces per thread for a width: up to 1024 columns a row stays within one wave (no barrier), beyond that 8 .. 16 values per lane
+template <class F>
 void by_width(int D, F go) {
-    if constexpr (VEC) {
-        if (D <= 64) return go(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
-        if (D <= 128) return go(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
-    }
-    if (D <= 256) go(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+    if (D <= 64) go(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    else if (D <= 128) go(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    else if (D <= 256) go(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
     else if (D <= 512) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
     else if (D <= 1024) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else if (D <= 2048) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    else if (D <= 2048) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
     else if (D <= 4096) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    else if (D <= 8192) go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 1>{});
+    else if (D <= 8192) go(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
 }
 
-template <class T, bool VEC>
-void launch_norm_tv(const NormArgs& a, int grid, bool backward, hipStream_t st) {
-    by_width<T, VEC>(a.D, [&](auto nt, auto nv) {
+template <class T, bool WHOLE>
+void launch_norm_t(const NormArgs& a, int grid, bool backward, hipStream_t st) {
+    by_width(a.D, [&](auto nt, auto nv) {
         constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
         const dim3 b(NT > 256 ? NT : 256);
-        if (backward) hipLaunchKernelGGL((norm_bwd_kernel<T, NT, NV, VEC>), dim3(grid), b, 0, st, a);
-        else hipLaunchKernelGGL((norm_fwd_kernel<T, NT, NV, VEC>), dim3(grid), b, 0, st, a);
+        if (backward) hipLaunchKernelGGL((norm_bwd_kernel<T, NT, NV, WHOLE>), dim3(grid), b, 0, st, a);
+        else hipLaunchKernelGGL((norm_fwd_kernel<T, NT, NV, WHOLE>), dim3(grid), b, 0, st, a);
     });
-}
-template <class T>
-void launch_norm_t(const NormArgs& a, bool vec, int grid, bool backward, hipStream_t st) {
-    if (vec) launch_norm_tv<T, true>(a, grid, backward, st);
-    else launch_norm_tv<T, false>(a, grid, backward, st);
 }
 
 }  // namespace
 
-int norm_rows_per_group(int D, bool vec) {
-    int r = 1;
-    auto f = [&](auto nt, auto) { constexpr int NT = decltype(nt)::value; r = NT >= 256 ? 1 : 256 / NT; };
-    if (vec) by_width<float, true>(D, f); else by_width<float, false>(D, f);
+int norm_threads(int D) {
+    int r = 0;
+    by_width(D, [&](auto nt, auto) { r = decltype(nt)::value > 256 ? decltype(nt)::value : 256; });
+    return r;
+}
+int norm_rows_per_group(int D) {
+    int r = 0;
+    by_width(D, [&](auto nt, auto) { r = decltype(nt)::value > 256 ? 1 : 256 / decltype(nt)::value; });
     return r;
 }
 
@@ -318,10 +349,11 @@ void launch_norm_join(int dtype, const float* part, int groups, int D, void* dw,
     else hipLaunchKernelGGL((norm_join_kernel<_Float16>), grid, dim3(256), 0, st, part, groups, D, dw, db, param_f32);
 }
 
-void launch_norm(int dtype, const NormArgs& a, bool vec, int grid, bool backward, hipStream_t st) {
-    if (dtype == 0) launch_norm_t<float>(a, vec, grid, backward, st);
-    else if (dtype == 1) launch_norm_t<__bf16>(a, vec, grid, backward, st);
-    else launch_norm_t<_Float16>(a, vec, grid, backward, st);
+void launch_norm(int dtype, const NormArgs& a, int grid, bool backward, hipStream_t st) {
+    const bool whole = a.D % 8 == 0;
+    if (dtype == 0) whole ? launch_norm_t<float, true>(a, grid, backward, st) : launch_norm_t<float, false>(a, grid, backward, st);
+    else if (dtype == 1) whole ? launch_norm_t<__bf16, true>(a, grid, backward, st) : launch_norm_t<__bf16, false>(a, grid, backward, st);
+    else whole ? launch_norm_t<_Float16, true>(a, grid, backward, st) : launch_norm_t<_Float16, false>(a, grid, backward, st);
 }
 
 }  // namespace ops
