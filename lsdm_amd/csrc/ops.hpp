@@ -36,17 +36,21 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
         for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
     }
 }
-template <class T>
+// STREAM: 16-bit results that nothing reads soon are stored non-temporally (norms 5 .. 15 %, products 3 .. 10 % of the time at large sizes: the inputs
+// keep the caches).  Not scratch memory that the next launch reads (its products lost 10 %), and not where a wave's store leaves gaps for a second one to
+// fill, as the two halves of an fp32 piece do: such lines are written twice (unpack8: 32 -> 63 us in bf16, 89 -> 311 us in fp32 at 32768 x 2048).
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    typedef typename Piece<T>::frag frag;
     typedef typename Piece<T>::mem mem;
-    if constexpr (sizeof(T) == 2) {
-        typename Piece<T>::frag r;
+    constexpr int H = 8 * (int)sizeof(T) / 16;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
-        *reinterpret_cast<mem*>(p) = r;
-    } else {
-        *reinterpret_cast<mem*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<mem*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    for (int k = 0; k < H; ++k) {
+        frag r;
+#pragma unroll
+        for (int j = 0; j < 8 / H; ++j) r[j] = (T)v[k * (8 / H) + j];
+        mem* q = reinterpret_cast<mem*>(p + k * (8 / H));
+        if constexpr (STREAM && sizeof(T) == 2) __builtin_nontemporal_store(r, q); else *q = r;
     }
 }
 // a piece cut short by the row's end: n valid elements (n <= 0: none); the others read as 0 and are not written
@@ -56,9 +60,9 @@ __device__ __forceinline__ void load8n(const T* p, int n, float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
 }
-template <class T>
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void store8n(T* p, int n, const float (&v)[8]) {
-    if (n >= 8) return store8(p, v);
+    if (n >= 8) return store8<STREAM>(p, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) if (j < n) p[j] = (T)v[j];
 }
@@ -93,41 +97,54 @@ __device__ __forceinline__ void store_param(void* p, int is_f32, long long i, fl
 // ---- activations: y = a(z) and, where asked for, d = a'(z) ----
 // fp32 results use the libm functions; 16-bit results the hardware exp2 / reciprocal forms of common.hpp (absolute error <= 3e-7, four orders
 // below a bf16 step of a value near one).  NaN stays NaN in y for every activation; relu'(NaN) = 0 (the comparison z > 0).
-template <class T>
-__device__ __forceinline__ void act_eval(int act, float z, bool want, float& y, float& d) {
+template <class T, int ACT>
+__device__ __forceinline__ void act_one(float z, bool want, float& y, float& d) {
     constexpr bool fast = sizeof(T) == 2;
-    d = 1.0f;
+    if constexpr (ACT == OP_RELU) {
+        y = z <= 0.0f ? 0.0f : z;
+        d = z > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == OP_GELU && fast) {
+        const float x = fabsf(z) * 0.70710678118654752440f;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f)), ex = __expf(-x * x);
+        float pl = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+        pl = fmaf(t, pl, 0.5f * 1.421413741f);
+        pl = fmaf(t, pl, 0.5f * -0.284496736f);
+        pl = fmaf(t, pl, 0.5f * 0.254829592f);
+        const float q = pl * t * ex, phi = z < 0.0f ? q : 1.0f - q;
+        y = z * phi;
+        d = fmaf(z * 0.39894228040143267794f, ex, phi);
+    } else if constexpr (ACT == OP_GELU) {
+        const float phi = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+        y = z * phi;
+        if (want) d = phi + z * 0.39894228040143267794f * expf(-0.5f * z * z);
+    } else if constexpr (ACT == OP_QUICK_GELU || ACT == OP_SILU) {
+        constexpr float c = ACT == OP_SILU ? 1.0f : 1.702f;
+        const float s = fast ? sigmoid_fast(c * z) : sigmoidf(c * z);
+        y = z * s;
+        d = s * fmaf(c * z, 1.0f - s, 1.0f);
+    } else if constexpr (ACT == OP_SIGMOID) {
+        y = fast ? sigmoid_fast(z) : sigmoidf(z);
+        d = y * (1.0f - y);
+    } else {
+        y = tanhf(z);
+        d = fmaf(-y, y, 1.0f);
+    }
+}
+template <class T, int ACT>
+__device__ __forceinline__ void act_each(const float (&z)[8], bool want, float (&y)[8], float (&d)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) act_one<T, ACT>(z[j], want, y[j], d[j]);
+}
+// one branch on the activation for eight values, whose chains of transcendentals then overlap
+template <class T>
+__device__ __forceinline__ void act8(int act, const float (&z)[8], bool want, float (&y)[8], float (&d)[8]) {
     switch (act) {
-        case OP_RELU: y = z <= 0.0f ? 0.0f : z; d = z > 0.0f ? 1.0f : 0.0f; break;
-        case OP_GELU: {
-            const float x = fabsf(z) * 0.70710678118654752440f;
-            if constexpr (fast) {
-                const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f)), ex = __expf(-x * x);
-                float pl = fmaf(t, 1.061405429f, -1.453152027f);
-                pl = fmaf(t, pl, 1.421413741f);
-                pl = fmaf(t, pl, -0.284496736f);
-                pl = fmaf(t, pl, 0.254829592f);
-                const float q = 0.5f * (pl * t) * ex, phi = z < 0.0f ? q : 1.0f - q;
-                y = z * phi;
-                d = fmaf(z * 0.39894228040143267794f, ex, phi);
-            } else {
-                const float phi = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
-                y = z * phi;
-                if (want) d = phi + z * 0.39894228040143267794f * expf(-0.5f * z * z);
-            }
-            break;
-        }
-        case OP_QUICK_GELU:
-        case OP_SILU: {
-            const float c = act == OP_SILU ? 1.0f : 1.702f;
-            const float s = fast ? sigmoid_fast(c * z) : sigmoidf(c * z);
-            y = z * s;
-            d = s * fmaf(c * z, 1.0f - s, 1.0f);
-            break;
-        }
-        case OP_SIGMOID: y = fast ? sigmoid_fast(z) : sigmoidf(z); d = y * (1.0f - y); break;
-        case OP_TANH: y = tanhf(z); d = fmaf(-y, y, 1.0f); break;
-        default: y = z; break;
+        case OP_RELU: act_each<T, OP_RELU>(z, want, y, d); break;
+        case OP_GELU: act_each<T, OP_GELU>(z, want, y, d); break;
+        case OP_QUICK_GELU: act_each<T, OP_QUICK_GELU>(z, want, y, d); break;
+        case OP_SILU: act_each<T, OP_SILU>(z, want, y, d); break;
+        case OP_SIGMOID: act_each<T, OP_SIGMOID>(z, want, y, d); break;
+        default: act_each<T, OP_TANH>(z, want, y, d); break;
     }
 }
 
@@ -179,6 +196,7 @@ struct Epilogue {
     void* out = nullptr; long long ldo = 0;
     void* deriv = nullptr; long long ldd = 0; int form = DERIV_NONE;   // a'(z) for the backward pass
     int act = OP_NONE;
+    int stream = 0;                                                 // rows of out and deriv are made of whole 128-byte lines
 };
 struct GemmArgs {
     const void *A = nullptr, *B = nullptr;                          // C(m, n) = sum_k A(m, k) B(n, k)

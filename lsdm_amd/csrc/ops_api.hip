@@ -103,11 +103,11 @@ GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
 
 int64_t part_bytes(const GemmPlan& p, int64_t M, int64_t N) { return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0; }
 
-// work-groups of a preparation pass: about 2048 in all, at least eight rows each
+// work-groups of a preparation pass: about 2048 in all, at least 32 rows each (four per thread, whose loads are in flight together)
 int prep_chunks(int64_t rows, int64_t cols) {
     const int64_t cb = (cols + 255) / 256;
     int64_t c = 2048 / cb;
-    if (c > (rows + 7) / 8) c = (rows + 7) / 8;
+    if (c > (rows + 31) / 32) c = (rows + 31) / 32;
     if (c > 1024) c = 1024;
     return c < 1 ? 1 : (int)c;
 }
@@ -158,6 +158,8 @@ PrepJob padded(int dtype, const void* src, int64_t lds, int64_t rows, int64_t n,
     j.src = src; j.lds = lds; j.dst = dst; j.ldd = ldd; j.rows = rows; j.n = (int)n; j.chunks = prep_chunks(rows, ldd);
     return j;
 }
+// rows made of whole 128-byte lines
+bool whole_lines(const void* p, int64_t width, int es) { return ((uintptr_t)p & 127) == 0 && width * es % 128 == 0; }
 int deriv_form(int dtype, int flags) { return flags & LSDM_OP_DERIV8 ? DERIV_8 : dtype == LSDM_F32 ? DERIV_F32 : DERIV_16; }
 
 int check_linear(int dtype, int64_t M, int64_t N, int64_t K) {
@@ -212,6 +214,7 @@ int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int
     e.out = y; e.ldo = N;
     e.act = activation;
     if (activation != LSDM_ACT_NONE && deriv) { e.deriv = deriv; e.ldd = N; e.form = deriv_form(dtype, flags); }
+    e.stream = whole_lines(y, N, es) && (!e.deriv || whole_lines(e.deriv, N, es));
     if (f.rows) {
         launch_rows(dtype, g, st);
         return launched("lsdm_linear");
@@ -275,7 +278,7 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
         g.M = (int)M; g.N = (int)K; g.K = (int)N;
         g.A = z; g.lda = ldz; g.B = ws_; g.ldb = ldws;
         g.part = b.partx;
-        g.e.out = dx; g.e.ldo = K;
+        g.e.out = dx; g.e.ldo = K; g.e.stream = whole_lines(dx, K, es);
         launch_gemm(dtype, b.px, g, KM, st);
     }
     if (dw) {
@@ -283,7 +286,7 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
         g.M = (int)N; g.N = (int)K; g.K = (int)M;
         g.A = z; g.lda = ldz; g.B = xs; g.ldb = ldxs;
         g.part = b.partw;
-        g.e.out = dw; g.e.ldo = K;
+        g.e.out = dw; g.e.ldo = K; g.e.stream = whole_lines(dw, K, es);
         launch_gemm(dtype, b.pw, g, MM, st);
     }
     return launched("lsdm_linear_backward");

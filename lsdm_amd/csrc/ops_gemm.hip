@@ -178,8 +178,7 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = z[j];
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) act_eval<T>(e.act, z[j], want, y[j], d[j]);
+        act8<T>(e.act, z, want, y, d);
         if (want) {
             if (e.form == DERIV_8) {
                 unsigned c[8];
@@ -195,7 +194,8 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
                     typename Piece<T>::frag f;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) f[j] = v[j];
-                    *reinterpret_cast<typename Piece<T>::mem*>(p) = f;
+                    typename Piece<T>::mem* q = reinterpret_cast<typename Piece<T>::mem*>(p);
+                    if (e.stream) __builtin_nontemporal_store(f, q); else *q = f;
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) if (j < cnt) p[j] = v[j];
@@ -210,7 +210,7 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, float (&z)[8], cons
         for (int j = 0; j < 8; ++j) y[j] += r[j];
     }
     T* p = static_cast<T*>(e.out) + m * e.ldo + n;
-    store8n(p, cnt, y);
+    if (e.stream) store8n<true>(p, cnt, y); else store8n(p, cnt, y);
 }
 template <class T>
 __device__ __forceinline__ void bias8(const Epilogue& e, int n, int N, float (&b)[8]) {
@@ -465,6 +465,46 @@ __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs g) {
 //   dst (rows, ldd) = src (rows, n) * d, or the values of an 8-bit checkpoint; columns n .. ldd - 1 are zeroed, so that rows no 16-byte load divides
 //   become rows that one does.  part[blockIdx.y][c] = the work-group's sum of the fp32 products over its rows (a fixed order).
 // Bound by HBM: each operand is read once, dst is written once.
+// one row's piece: v = the source's values times a'(z).  Whole pieces are loaded outside any branch on the lane, so that several rows' are in flight.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void prep_piece(const PrepJob& a, long long r, int c0, int n, float (&v)[8]) {
+    typedef typename Piece<T>::frag frag;
+    typedef typename Piece<T>::mem mem;
+    const long long at = r * a.n + c0;
+    if (a.exps) {
+        const unsigned char* q = static_cast<const unsigned char*>(a.src) + at;
+        const u32x2 w = WHOLE ? *reinterpret_cast<const codes8*>(q) : load_codes(q, n);
+        const float step = n > 0 ? exp8_step(a.exps[r * ((a.n + 31) >> 5) + (c0 >> 5)]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)((int)(w[j >> 2] << (24 - 8 * (j & 3))) >> 24) * step;
+    } else {
+        const T* p = static_cast<const T*>(a.src) + r * a.lds + c0;
+        if constexpr (WHOLE) load8(p, v); else load8n(p, n, v);
+    }
+    if (a.form == DERIV_NONE) return;
+    float d[8];
+    if (a.form == DERIV_8) {
+        const unsigned char* q = static_cast<const unsigned char*>(a.deriv) + at;
+        const u32x2 w = WHOLE ? *reinterpret_cast<const codes8*>(q) : load_codes(q, n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = deriv_value8((w[j >> 2] >> (8 * (j & 3))) & 255u);
+    } else if constexpr (sizeof(T) == 2) {
+        const T* q = static_cast<const T*>(a.deriv) + at;
+        if constexpr (WHOLE) {
+            const frag f = *reinterpret_cast<const mem*>(q);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] = deriv_value16(__builtin_bit_cast(unsigned short, (T)f[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value16(__builtin_bit_cast(unsigned short, q[j])) : 0.0f;
+        }
+    } else {
+        const float* q = static_cast<const float*>(a.deriv) + at;
+        if constexpr (WHOLE) load8(q, d); else load8n(q, n, d);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = WHOLE || j < n ? v[j] * d[j] : 0.0f;
+}
 template <class T>
 __global__ __launch_bounds__(256) void prep_kernel(PrepArgs args) {
     const PrepJob& a = args.job[blockIdx.z];
@@ -474,44 +514,33 @@ __global__ __launch_bounds__(256) void prep_kernel(PrepArgs args) {
     if ((int)blockIdx.y >= a.chunks || (long long)blockIdx.x * 256 >= (a.dst && a.ldd > a.n ? a.ldd : a.n)) return;      // (whole work-groups)
     const long long per = (a.rows + a.chunks - 1) / a.chunks, lo = (long long)blockIdx.y * per, hi = min(a.rows, lo + per);
     const int n = max(0, min(8, a.n - c0));
-    const int gpr = (a.n + 31) >> 5;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (n > 0 || (a.dst && c0 < a.ldd)) {
-#pragma unroll 2
+    T* dst = static_cast<T*>(a.dst) + c0;
+    if (n == 8) {
+        long long r = lo + tr;
+        for (; r + 24 < hi; r += 32) {
+            float v[4][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) prep_piece<T, true>(a, r + 8 * u, c0, 8, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (a.dst) store8(dst + (r + 8 * u) * a.ldd, v[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] += v[u][j];
+            }
+        }
+        for (; r < hi; r += 8) {
+            float v[8];
+            prep_piece<T, true>(a, r, c0, 8, v);
+            if (a.dst) store8(dst + r * a.ldd, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] += v[j];
+        }
+    } else if (n > 0 || (a.dst && c0 < a.ldd)) {
         for (long long r = lo + tr; r < hi; r += 8) {
-            float v[8], d[8];
-            if (a.exps) {
-                const signed char* q = static_cast<const signed char*>(a.src) + r * a.n + c0;
-                const float step = n > 0 ? exp8_step(a.exps[r * gpr + (c0 >> 5)]) : 0.0f;
-                const u32x2 w = load_codes(q, n);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (float)((int)(w[j >> 2] << (24 - 8 * (j & 3))) >> 24) * step;
-            } else {
-                load8n(static_cast<const T*>(a.src) + r * a.lds + c0, n, v);
-            }
-            if (a.form != DERIV_NONE) {
-                const long long at = r * a.n + c0;
-                if (a.form == DERIV_8) {
-                    const u32x2 w = load_codes(static_cast<const unsigned char*>(a.deriv) + at, n);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) d[j] = deriv_value8((w[j >> 2] >> (8 * (j & 3))) & 255u);
-                } else if constexpr (sizeof(T) == 2) {
-                    const T* q = static_cast<const T*>(a.deriv) + at;
-                    if (n >= 8) {
-                        const typename Piece<T>::frag f = *reinterpret_cast<const typename Piece<T>::mem*>(q);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] = deriv_value16(__builtin_bit_cast(unsigned short, (T)f[j]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] = j < n ? deriv_value16(__builtin_bit_cast(unsigned short, q[j])) : 0.0f;
-                    }
-                } else {
-                    load8n(static_cast<const float*>(a.deriv) + at, n, d);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] * d[j] : 0.0f;
-            }
-            if (a.dst && c0 < a.ldd) store8(static_cast<T*>(a.dst) + r * a.ldd + c0, v);
+            float v[8];
+            prep_piece<T, false>(a, r, c0, n, v);
+            if (a.dst) store8(dst + r * a.ldd, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) s[j] += v[j];
         }

@@ -99,7 +99,7 @@ __device__ __forceinline__ void row_store(T* p, int D, int l, const float (&v)[N
     for (int i = 0; i < NV; ++i) {
         const int c = col_of<NT>(l, i);
         if (c < D) {
-            if constexpr (WHOLE) store8(p + c, v[i]); else store8n(p + c, D - c, v[i]);
+            if constexpr (WHOLE) store8<true>(p + c, v[i]); else store8n<true>(p + c, D - c, v[i]);
         }
     }
 }

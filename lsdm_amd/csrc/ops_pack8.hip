@@ -16,8 +16,13 @@ __global__ __launch_bounds__(256) void pack8_kernel(Pack8Args a, long long halve
     const int h = (int)(i - r * hpr), c = h * 16, n = a.D - c;
     float v[2][8];
     const T* p = static_cast<const T*>(a.x) + r * a.ldx + c;
-    load8n(p, n, v[0]);
-    load8n(p + 8, n - 8, v[1]);
+    if (n >= 16) {                               // (both pieces in one branch: two loads in flight)
+        load8(p, v[0]);
+        load8(p + 8, v[1]);
+    } else {
+        load8n(p, n, v[0]);
+        load8n(p + 8, n - 8, v[1]);
+    }
     unsigned m = 0;
 #pragma unroll
     for (int k = 0; k < 16; ++k) m = max(m, __builtin_bit_cast(unsigned, v[k >> 3][k & 7]) & 0x7fffffffu);
