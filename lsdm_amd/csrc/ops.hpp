@@ -153,8 +153,8 @@ __device__ __forceinline__ void act8(int act, const float (&z)[8], bool want, fl
 // absolute below, a sixteenth (bf16) and a quarter (fp16) of the type's own rounding.  The bits are fp32's after a scaling by 2^-120, which makes
 // the exponent field of [1, 2) a 7.  0x7fff stands for NaN.
 __device__ __forceinline__ unsigned deriv_code16(float d) {
-    const unsigned b = __builtin_bit_cast(unsigned, fabsf(d) * 0x1p-120f), s = (__builtin_bit_cast(unsigned, d) >> 16) & 0x8000u;
-    return d != d ? 0x7fffu : (s | (b + 0x3ffu + ((b >> 11) & 1u)) >> 11);
+    const unsigned b = __builtin_bit_cast(unsigned, d * 0x1p-120f);
+    return min(((b & 0x7fffffffu) + 0x400u) >> 11, 0x7fffu) | ((b >> 16) & 0x8000u);      // (nearest, ties upwards; a NaN's bits end at the limit)
 }
 __device__ __forceinline__ float deriv_value16(unsigned u) {
     const float v = __builtin_bit_cast(float, (u & 0x7fffu) << 11) * 0x1p120f;

@@ -103,11 +103,14 @@ GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
 
 int64_t part_bytes(const GemmPlan& p, int64_t M, int64_t N) { return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0; }
 
-// work-groups of a preparation pass: about 2048 in all, at least 32 rows each (four per thread, whose loads are in flight together)
+// row chunks of a preparation job: about 2048 work-groups in all with at least 32 rows each (four per thread, whose loads are in flight together); fewer
+// rows where there would be less than a work-group for every CU.  The column sums' join reads one row per chunk.
 int prep_chunks(int64_t rows, int64_t cols) {
-    const int64_t cb = (cols + 255) / 256;
-    int64_t c = 2048 / cb;
-    if (c > (rows + 31) / 32) c = (rows + 31) / 32;
+    const int64_t cb = (cols + 255) / 256, most = (rows + 7) / 8;
+    int64_t c = (rows + 31) / 32, fill = (kCUs + cb - 1) / cb;
+    if (fill > most) fill = most;
+    if (c < fill) c = fill;
+    if (c > 2048 / cb) c = 2048 / cb;
     if (c > 1024) c = 1024;
     return c < 1 ? 1 : (int)c;
 }

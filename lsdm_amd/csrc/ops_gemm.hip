@@ -223,7 +223,7 @@ template <class T>
 __device__ __forceinline__ void colsum_join(const GemmArgs& g, int block, float* red) {
     const int t = threadIdx.x, c = block * 64 + (t & 63), q = t >> 6, nw = (int)blockDim.x >> 6;
     float s = 0.0f;
-    if (c < g.cs_n)
+    if (c < g.cs_n)                              // (sixteen loads in flight: the products' tiles must not wait for this work-group)
 #pragma unroll 4
         for (int k = q; k < g.cs_chunks; k += nw) s += g.cs_part[(long long)k * g.cs_n + c];
     red[t] = s;
@@ -537,6 +537,7 @@ __global__ __launch_bounds__(256) void prep_kernel(PrepArgs args) {
             for (int j = 0; j < 8; ++j) s[j] += v[j];
         }
     } else if (n > 0 || (a.dst && c0 < a.ldd)) {
+#pragma unroll 4
         for (long long r = lo + tr; r < hi; r += 8) {
             float v[8];
             prep_piece<T, false>(a, r, c0, n, v);

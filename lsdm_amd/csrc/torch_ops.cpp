@@ -72,7 +72,11 @@ Tensor maybe_contiguous(const Tensor& t) { return t.defined() ? t.contiguous() :
 void check_capture(const char* who, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
     const auto current = c10::hip::getCurrentHIPStream(x.device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess) {       // (the default stream while another one is captured)
+        (void)hipGetLastError();
+        return;
+    }
+    if (status == hipStreamCaptureStatusNone) return;
     for (const Tensor* t : inputs) {
         if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
