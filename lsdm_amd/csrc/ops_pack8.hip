@@ -1,6 +1,7 @@
 // 8-bit activation checkpoints (ops.hpp: the format; include/lsdm_hip.h: lsdm_pack8, lsdm_unpack8), gfx950.  Bound by HBM: pack reads a value and
 // writes 33/32 bytes, unpack the reverse.
 // A thread owns 16 consecutive values of a row; two threads share a group and its maximum by one cross-lane exchange.
+// Measured: 32768 x 2048 bf16 pack 31 us, unpack 32 us (6.6 TB/s, part of it out of the cache); fp32 59 and 91 us.
 #include "ops.hpp"
 #include "ops_launch.hpp"
 
