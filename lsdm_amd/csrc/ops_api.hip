@@ -70,7 +70,7 @@ struct Carve {
 // are written once and read once).  The constants are fitted to 1400 timed launches (135 shapes log-uniform over 16 .. 16384, every tile, 1 .. 32
 // splits, three operand layouts): the estimate's choice is within 1 % of the best one in the mean, within 16 % at worst.
 struct TileCost { int tile, resident; float alone, shared, fixed, each; };
-const TileCost kHalfTiles[] = {{256, 1, 0.0f, 1.44f, 8.8f, 0.6f}, {128, 2, 0.68f, 0.40f, 2.1f, 1.55f}, {64, 5, 0.31f, 0.18f, 2.7f, 0.07f}};
+const TileCost kHalfTiles[] = {{256, 1, 0.0f, 1.36f, 8.8f, 0.6f}, {128, 2, 0.68f, 0.40f, 2.1f, 1.55f}, {64, 5, 0.31f, 0.18f, 2.7f, 0.07f}};
 const TileCost kSingleTiles[] = {{128, 2, 0.40f, 1.61f, 4.9f, 0.13f}, {64, 4, 0.52f, 0.49f, 0.06f, 0.09f}};
 constexpr float kJoinLaunch = 2.6f, kJoinBytesPerUs = 3.6e6f;
 

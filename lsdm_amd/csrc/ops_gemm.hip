@@ -15,7 +15,7 @@
 // the reader.  A lane whose k lies beyond the end reads 16 zero bytes (g_zero16); rows beyond the end are clamped to the last one, and their
 // results are not stored.
 // Measured (MI355X, back to back): 8192 x 4096 x 8256 bf16 KK 428 us = 1.30 PFLOP/s (a 16 KiB row stride, K = 8192, costs 15 %: the rows of a tile fall on
-// the same channels), 16384 x 2048 x 8192 KM 468 us = 1.18, 8192 x 2048 x 16384 MM 450 us = 1.22; fp32 4096^3 KM 1.05 ms = 0.131.  Bound by the issue of
+// the same channels), 16384 x 2048 x 8192 KM 448 us = 1.23, 8192 x 2048 x 8192 MM 203 us = 1.36; fp32 4096^3 KM 1.05 ms = 0.131.  Bound by the issue of
 // the LDS copies next to the matrix instructions (SQ_VALU_MFMA_BUSY 57 % of the cycles); with all rows on one cache line the same loop reaches 1.38.
 // Two 128-byte steps in flight; 64-byte steps three to five deep, or two groups of waves half a period apart, measured 0 .. 15 % slower.
 #include <algorithm>
@@ -328,6 +328,20 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
                     for (int j = 0; j < FN; ++j) acc[i][j] = MM_::go(fb[j], fa[i], acc[i][j], q);
+        }
+        if constexpr (sizeof(T) == 2 && (BM == 256 || (BM == 128 && !AKM))) {
+            // The compiler's own order reads a fragment, waits for it and uses it; this one starts with the B fragments and two of A and keeps every later
+            // read that far ahead of its use (256: KK 595 -> 573 us at 16384 x 2048 x 8192, KM 229 -> 214, MM 229 -> 211 at 8192 x 4096 x 4096; 128 MM 253 -> 236,
+            // but 128 KK and KM 3 .. 5 % slower, 64 the same: not there).
+            constexpr int RA = AKM ? 1 : 2, RB = BKM ? 1 : 2, READS = KS * (FM * RA + FN * RB), AHEAD = FN * RB + 2 * RA, MF = KS * FM * FN;
+            constexpr int PERR = MF / (READS - AHEAD);
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);            // LDS reads
+#pragma unroll
+            for (int g = 0; g < READS - AHEAD; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x8, PERR, 0);           // matrix instructions
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, MF - PERR * (READS - AHEAD), 0);
         }
         buf = buf + 1 == STAGES ? 0 : buf + 1;
     }
