@@ -10,9 +10,10 @@ of ``nn.Linear`` and ``nn.LayerNorm`` -- in place: parameters, names and ``state
 
 ``SceneDiffusionModel(..., text_kernels=True)`` does it for the tower the model loads itself.  What a block lets be fused is: BERT's
 ``dense -> activation`` and ``dense -> + input -> LayerNorm``, its pooler, and CLIP's ``x + c_proj(gelu(c_fc(ln_2(x))))``; everything else is replaced
-layer by layer, and attention itself stays with the package.
+layer by layer, and attention itself stays with the package.  Autocast does not reach the operators: give the tower the type instead (a call that mixes
+types raises ``ValueError``).
 """
-import types
+import functools
 
 import torch.nn as nn
 
@@ -21,6 +22,12 @@ from . import ops
 # activation modules whose function ops.linear has in its epilogue
 _ACT_BY_CLASS = {"GELUActivation": "gelu", "GELU": "gelu", "QuickGELU": "quick_gelu", "QuickGELUActivation": "quick_gelu", "SiLU": "silu", "SiLUActivation": "silu",
                  "ReLU": "relu", "Sigmoid": "sigmoid", "Tanh": "tanh"}
+
+
+# the blocks that are fused, by class and children
+_BLOCKS = {"BertIntermediate": {"dense", "intermediate_act_fn"}, "BertSelfOutput": {"dense", "LayerNorm", "dropout"}, "BertOutput": {"dense", "LayerNorm", "dropout"},
+           "BertPooler": {"dense", "activation"}, "ResidualAttentionBlock": {"attn", "ln_1", "mlp", "ln_2"}}
+_DENSE = ("dense", "c_fc", "c_proj")
 
 
 def _activation_name(module):
@@ -65,8 +72,12 @@ def _clip_block(self, x):
 
 
 def _fuse(module):
-    """Replaces the ``forward`` of a block whose layers form one of the fused patterns."""
-    name = type(module).__name__
+    """Replaces the ``forward`` of a block whose layers form one of the fused patterns: exactly these children, the dense layers among them replaced above (a
+    subclass of ``nn.Linear``, or a further layer in the block, keeps the block's own ``forward``)."""
+    name, children = type(module).__name__, dict(module.named_children())
+    mlp = dict(children["mlp"].named_children()) if "mlp" in children else {}
+    if set(children) != _BLOCKS.get(name) or any(type(c) is not Linear for n, c in [*children.items(), *mlp.items()] if n in _DENSE):
+        return
     if name == "BertIntermediate":
         act = _activation_name(module.intermediate_act_fn)
         forward = _dense_act
@@ -74,13 +85,13 @@ def _fuse(module):
         act, forward = "none", _dense_residual_norm
     elif name == "BertPooler":
         act, forward = _activation_name(module.activation), _pooler
-    elif name == "ResidualAttentionBlock" and hasattr(module, "attention") and all(hasattr(getattr(module, "mlp", None), n) for n in ("c_fc", "gelu", "c_proj")):
+    elif name == "ResidualAttentionBlock" and hasattr(module, "attention") and list(mlp) == ["c_fc", "gelu", "c_proj"]:
         act, forward = _activation_name(module.mlp.gelu), _clip_block
     else:
         return
     if act is not None:
         module._kernel_activation = act
-        module.forward = types.MethodType(forward, module)
+        module.forward = functools.partial(forward, module)       # (copies and pickles with the module, as a bound method would not)
 
 
 def use_kernels(tower, *, checkpoint8=False):

@@ -2,8 +2,10 @@
 the evaluation: u = 2^-24 for an fp32 operation, half a step of the result's type for the one rounding at the end, and the stated steps of what is kept
 for the backward pass.  Sums: a contraction of K terms is a chain of K fp32 additions in the worst order (2 K u sum |terms|); a row sum of the norm is
 at most 16 additions per lane and 10 across lanes and waves (32 u sum |terms|)."""
+import copy
 import ctypes as C
 import math
+import pickle
 
 import pytest
 import torch
@@ -795,6 +797,37 @@ def test_use_kernels_replaces_layers_in_place():
     kept = torch.nn.Sequential(torch.nn.LayerNorm([3, 4]), torch.nn.Linear(4, 4))
     use_kernels(kept)
     assert type(kept[0]) is torch.nn.LayerNorm                           # a norm over several axes is not the operator
+
+
+class Scaled(torch.nn.Linear):
+    """A dense layer of a user's own kind (adapters, quantised layers)."""
+    def forward(self, x):
+        return 2.0 * super().forward(x)
+
+
+def test_blocks_that_are_not_the_fused_pattern_keep_their_forward():
+    m = bert(layers=1)
+    layer = m.encoder.layer[0]
+    layer.intermediate.dense.__class__ = Scaled
+    layer.output.dense.__class__ = Scaled
+    m.pooler.extra = torch.nn.Identity()
+    use_kernels(m)
+    assert "forward" in vars(layer.attention.output) and type(layer.intermediate.dense) is Scaled
+    assert not any("forward" in vars(b) for b in (layer.intermediate, layer.output, m.pooler))
+    b = clip_block()
+    b.ls_1 = torch.nn.Identity()                                         # a scale on a branch
+    c = clip_block()
+    c.mlp.c_proj.__class__ = Scaled
+    d = clip_block()
+    d.mlp.add_module("drop", torch.nn.Dropout(0.5))
+    assert not any("forward" in vars(use_kernels(v)) for v in (b, c, d)) and "forward" in vars(use_kernels(clip_block()))
+
+
+def test_a_tower_on_the_operators_can_be_copied_and_pickled():
+    m = use_kernels(bert(layers=1))
+    for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        block, own = m.encoder.layer[0].intermediate, other.encoder.layer[0].intermediate
+        assert type(own.dense) is Linear and own.dense is not block.dense and own.forward.args[0] is own and torch.equal(own.dense.weight, block.dense.weight)
 
 
 @gpu
