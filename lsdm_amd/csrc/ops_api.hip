@@ -44,8 +44,9 @@ int launched(const char* what) {
 }
 
 constexpr int64_t kMaxSize = (int64_t)1 << 30;
+constexpr int64_t kMaxOut = (int64_t)1 << 25;     // rows of W: a launch's work-groups go with them, up to 1024 threads for every 16 of them
 constexpr int kCUs = 256;                         // MI355X
-constexpr int64_t kMaxTiles = (int64_t)1 << 30;   // work-groups of a launch
+constexpr int64_t kMaxThreads = (int64_t)1 << 31; // threads of a launch (the runtime takes fewer than 2^32; column-sum work-groups may come on top)
 int esize(int dtype) { return dtype == LSDM_F32 ? 4 : 2; }
 bool dtype_ok(int d) { return d == LSDM_F32 || d == LSDM_BF16 || d == LSDM_F16; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -83,9 +84,10 @@ GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
     for (int i = 0; i < kinds; ++i) {
         const TileCost& k = f32 ? kSingleTiles[i] : kHalfTiles[i];
         const int64_t tm = (M + k.tile - 1) / k.tile, tn = (N + k.tile - 1) / k.tile;
-        if (tm * tn > kMaxTiles) continue;
+        const int64_t most = kMaxThreads / (k.tile == 256 ? 512 : 256);
+        if (tm * tn > most) continue;
         for (int s = 1; s <= 32; s = s < 4 ? s + 1 : s * 2) {
-            if (s > 1 && (steps < 2 * s || tm * tn * s > kMaxTiles)) break;
+            if (s > 1 && (steps < 2 * s || tm * tn * s > most || M * ((N + 7) / 8) > kMaxThreads)) break;      // (the join: a thread per eight outputs)
             const int64_t per = (steps + s - 1) / s;
             if ((steps + per - 1) / per != s) continue;
             const int64_t groups = tm * tn * s, round = (int64_t)kCUs * k.resident, full = groups / round, rest = groups - full * round;
@@ -167,8 +169,8 @@ int deriv_form(int dtype, int flags) { return flags & LSDM_OP_DERIV8 ? DERIV_8 :
 
 int check_linear(int dtype, int64_t M, int64_t N, int64_t K) {
     if (!dtype_ok(dtype)) return refuse(LSDM_ERR_ARG, "lsdm_linear: unknown dtype %d", dtype);
-    if (M < 1 || N < 1 || K < 1 || M > kMaxSize || N > kMaxSize || K > kMaxSize)
-        return refuse(LSDM_ERR_ARG, "lsdm_linear: sizes (%lld, %lld, %lld) must lie in [1, 2^30]", (long long)M, (long long)N, (long long)K);
+    if (M < 1 || N < 1 || K < 1 || M > kMaxSize || N > kMaxOut || K > kMaxSize)
+        return refuse(LSDM_ERR_ARG, "lsdm_linear: sizes M = %lld, K = %lld must lie in [1, 2^30], N = %lld in [1, 2^25]", (long long)M, (long long)K, (long long)N);
     return LSDM_OK;
 }
 
@@ -344,8 +346,11 @@ int lsdm_layer_norm_backward(int device, int dtype, int flags, int64_t rows, int
     return launched("lsdm_layer_norm_backward");
 }
 
+// two threads per group of 32 values
+static bool pack8_sizes(int64_t rows, int64_t D) { return rows >= 1 && D >= 1 && D <= kMaxSize && rows <= kMaxThreads / ((D + 31) / 32 * 2); }
+
 int lsdm_pack8(int device, int dtype, int64_t rows, int64_t D, const void* x, int64_t ldx, void* codes, void* exps, void* stream) {
-    if (!dtype_ok(dtype) || rows < 1 || D < 1 || D > kMaxSize || !x || !codes || !exps || ldx < D) return refuse(LSDM_ERR_ARG, "lsdm_pack8: bad argument");
+    if (!dtype_ok(dtype) || !pack8_sizes(rows, D) || !x || !codes || !exps || ldx < D) return refuse(LSDM_ERR_ARG, "lsdm_pack8: bad argument");
     OnDevice dev(device);
     if (!dev.ok) return LSDM_ERR_HIP;
     Pack8Args a;
@@ -355,7 +360,7 @@ int lsdm_pack8(int device, int dtype, int64_t rows, int64_t D, const void* x, in
 }
 
 int lsdm_unpack8(int device, int dtype, int64_t rows, int64_t D, const void* codes, const void* exps, void* out, void* stream) {
-    if (!dtype_ok(dtype) || rows < 1 || D < 1 || D > kMaxSize || !codes || !exps || !out) return refuse(LSDM_ERR_ARG, "lsdm_unpack8: bad argument");
+    if (!dtype_ok(dtype) || !pack8_sizes(rows, D) || !codes || !exps || !out) return refuse(LSDM_ERR_ARG, "lsdm_unpack8: bad argument");
     OnDevice dev(device);
     if (!dev.ok) return LSDM_ERR_HIP;
     Pack8Args a;

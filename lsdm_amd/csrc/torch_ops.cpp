@@ -15,7 +15,7 @@ using torch::autograd::variable_list;
 
 struct LsdmFailure : std::runtime_error { using std::runtime_error::runtime_error; };      // becomes lsdm_amd._lib.LsdmError
 
-constexpr int64_t kMaxSize = (int64_t)1 << 30;
+constexpr int64_t kMaxSize = (int64_t)1 << 30, kMaxOut = (int64_t)1 << 25;
 constexpr int64_t kNormMaxWidth = 16384;
 
 template <class... A>
@@ -56,7 +56,7 @@ void check_device(const char* who, const char* name, const Tensor& t, const Tens
 // rows of `width` elements with unit stride and one row stride; copies only what no row stride can describe
 struct Rows { Tensor t; int64_t ld; };
 Rows rows_of(const Tensor& t, int64_t width) {
-    Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / width, width});
+    Tensor r = (t.dim() == 2 ? t : t.reshape({t.numel() / width, width})).resolve_neg();       // (a lazily negated view: z.conj().imag)
     if (r.stride(1) == 1 && r.stride(0) >= width) return {r, r.stride(0)};
     return {r.contiguous(), width};
 }
@@ -65,7 +65,7 @@ bool unaligned(const Rows& r, int64_t width) {
     return ((reinterpret_cast<int64_t>(r.t.data_ptr()) | r.ld * es | width * es) & 15) != 0;
 }
 Tensor scratch(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
-Tensor maybe_contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor maybe_contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 
 // A leaf whose gradient node is alive and sits on the default stream cannot take part in a capture on another stream: autograd would have to join
 // the default stream to it, and the failure surfaces where the process cannot recover.  Refused before anything is recorded.
@@ -236,7 +236,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bia
     if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1)) value_error("linear: expected x (..., K) and weight (N, K), got ", x.sizes(), " and ", w.sizes());
     const int64_t N = w.size(0), K = w.size(1);
     if (K < 1) value_error("linear: weight has no columns");
-    if (x.numel() / K > kMaxSize || N > kMaxSize || K > kMaxSize) value_error("linear: at most 2^30 rows and columns");
+    if (x.numel() / K > kMaxSize || N > kMaxOut || K > kMaxSize) value_error("linear: x holds at most 2^30 rows and columns, weight 2^25 rows");
     if (w.scalar_type() != x.scalar_type() || (residual.defined() && residual.scalar_type() != x.scalar_type()))
         value_error("linear: weight and residual must have x's dtype ", x.scalar_type());
     if (bias.defined() && (bias.dim() != 1 || bias.size(0) != N || (bias.scalar_type() != x.scalar_type() && bias.scalar_type() != at::kFloat)))

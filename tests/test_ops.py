@@ -252,6 +252,23 @@ def test_linear_layouts_and_leading_axes():
 
 
 @gpu
+def test_lazily_negated_views():
+    """torch keeps a conjugate's imaginary part as a view with a negation still to be done."""
+    x, w, b, r, dy = (t.contiguous() for t in linear_case(70, 40, 24, "f32", 3))
+    neg = torch._neg_view
+    assert neg(x).is_neg()
+    assert torch.equal(ops.linear(neg(x), neg(w), neg(b), "gelu", neg(r)), ops.linear(-x, -w, -b, "gelu", -r))
+    assert torch.equal(ops.layer_norm(neg(x), neg(w[0]), neg(w[1])), ops.layer_norm(-x, -w[0], -w[1]))
+    assert torch.equal(ops.checkpoint8(neg(x)).restore(), ops.checkpoint8(-x).restore())
+    for f in (lambda t: ops.linear(t, w, b, "gelu"), lambda t: ops.layer_norm(t)):
+        t = x.clone().requires_grad_()
+        y = f(t)
+        g = dy if y.shape == dy.shape else x
+        want, got = torch.autograd.grad(y, t, -g, retain_graph=True)[0], torch.autograd.grad(y, t, neg(g))[0]
+        assert torch.equal(got, want)
+
+
+@gpu
 def test_linear_subsets_of_gradients():
     x, w, b, r, dy = linear_case(90, 40, 24, "bf16", 4)
     for need in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 1, 0), (0, 1, 0, 1)):
@@ -716,6 +733,12 @@ def test_c_entries_refuse_bad_arguments_before_they_touch_a_device():
     bad(lib.lsdm_layer_norm_backward(0, 1, 0, 4, 8, P, 8, P, 8, None, None, None, P, P, P, P, None, None, 0, None), "workspace")
     bad(lib.lsdm_pack8(0, 1, 0, 8, P, 8, P, P, None), "pack8")
     bad(lib.lsdm_unpack8(0, 5, 1, 8, P, P, P, None), "unpack8")
+    bad(lin(N=(1 << 25) + 1, r=P, ldr=1 << 26), "sizes")
+    bad(lib.lsdm_pack8(0, 1, 1 << 31, 32, P, 32, P, P, None), "pack8")
+    bad(lib.lsdm_unpack8(0, 1, 1 << 31, 32, P, P, P, None), "unpack8")
+    # sizes whose tiles are more threads than a launch takes choose a larger tile, or are refused
+    assert lib.lsdm_linear_workspace(0, 0, 1 << 30, 1, 8) == 0
+    bad(lin(dt=0, M=1 << 30, N=1 << 20, ldw=8), "tiles")
     assert lib.lsdm_linear_workspace(1, 0, 0, 8, 8) == -1 and lib.lsdm_layer_norm_workspace(4, 0) == -1
     assert lib.lsdm_linear_workspace(1, 0, 64, 8, 7) == 0 and lib.lsdm_linear_workspace(1, 0, 1000, 512, 512) >= 0
 
