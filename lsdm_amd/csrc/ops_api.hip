@@ -68,22 +68,24 @@ struct Carve {
 // Tile and split of C (M, N) with contraction K, by an estimate of the launch's time.  A tile kind keeps up to `resident` work-groups on a CU; a
 // 128-byte step of the contraction takes max(alone, shared * n) us with n of them there, prologue and epilogue fixed + each * n us.  The grid runs
 // in full rounds of 256 `resident` work-groups and a last, thinner one; a split contraction adds the join's launch and its traffic (the partial sums
-// are written once and read once).  The constants are fitted to 1400 timed launches (135 shapes log-uniform over 16 .. 16384, every tile, 1 .. 32
-// splits, three operand layouts): the estimate's choice is within 1 % of the best one in the mean, within 16 % at worst.
-struct TileCost { int tile, resident; float alone, shared, fixed, each; };
-const TileCost kHalfTiles[] = {{256, 1, 0.0f, 1.36f, 8.8f, 0.6f}, {128, 2, 0.68f, 0.40f, 2.1f, 1.55f}, {64, 5, 0.31f, 0.18f, 2.7f, 0.07f}};
-const TileCost kSingleTiles[] = {{128, 2, 0.40f, 1.61f, 4.9f, 0.13f}, {64, 4, 0.52f, 0.49f, 0.06f, 0.09f}};
+// are written once and read once).  The constants are fitted to timed launches of every tile and 1 .. 32 splits in the three operand layouts (16 bits:
+// 177 shapes log-uniform over 16 .. 16384; fp32: 35): the estimate's choice is within 1 % of the best one in the mean, within 20 % at worst.  Without
+// the 64 x 128 tile it would be 1.5 % (4928 x 2048 x 512: 22 -> 18 us, 704 x 1640 x 3952: 37 -> 25).
+struct TileCost { int tile, tile_n, resident; float alone, shared, fixed, each; };
+const TileCost kHalfTiles[] = {{256, 256, 1, 0.0f, 1.36f, 8.5f, 0.61f}, {128, 128, 2, 0.78f, 0.39f, 1.87f, 1.4f}, {64, 128, 3, 0.395f, 0.28f, 1.98f, 0.74f},
+                               {64, 64, 5, 0.315f, 0.19f, 2.31f, 0.08f}};
+const TileCost kSingleTiles[] = {{128, 128, 2, 0.40f, 1.61f, 4.9f, 0.13f}, {64, 64, 4, 0.52f, 0.49f, 0.06f, 0.09f}};
 constexpr float kJoinLaunch = 2.6f, kJoinBytesPerUs = 3.6e6f;
 
 GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
     const bool f32 = dtype == LSDM_F32;
-    const int bk = f32 ? 32 : 64, kinds = f32 ? 2 : 3;
+    const int bk = f32 ? 32 : 64, kinds = f32 ? 2 : 4;
     const int64_t steps = (K + bk - 1) / bk;
     GemmPlan best;
     float best_us = 0.0f;
     for (int i = 0; i < kinds; ++i) {
         const TileCost& k = f32 ? kSingleTiles[i] : kHalfTiles[i];
-        const int64_t tm = (M + k.tile - 1) / k.tile, tn = (N + k.tile - 1) / k.tile;
+        const int64_t tm = (M + k.tile - 1) / k.tile, tn = (N + k.tile_n - 1) / k.tile_n;
         const int64_t most = kMaxThreads / (k.tile == 256 ? 512 : 256);
         if (tm * tn > most) continue;
         for (int s = 1; s <= 32; s = s < 4 ? s + 1 : s * 2) {
@@ -96,7 +98,7 @@ GemmPlan plan(int64_t M, int64_t N, int64_t K, int dtype) {
             if (s > 1) us += kJoinLaunch + (float)(s + 1) * (float)M * (float)N * 4.0f / kJoinBytesPerUs;
             if (best.tile == 0 || us < best_us) {
                 best_us = us;
-                best.tile = k.tile; best.tiles_m = (int)tm; best.tiles_n = (int)tn; best.splits = s; best.kchunk = (int)(per * bk);
+                best.tile = k.tile; best.tile_n = k.tile_n; best.tiles_m = (int)tm; best.tiles_n = (int)tn; best.splits = s; best.kchunk = (int)(per * bk);
             }
         }
     }

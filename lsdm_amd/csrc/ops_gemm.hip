@@ -597,9 +597,10 @@ void launch_gemm_t(const GemmPlan& p, GemmArgs g, int layout, hipStream_t st) {
     const unsigned grid = (unsigned)(g.blocks + (g.cs_out ? (g.cs_n + 63) / 64 : 0));
     if constexpr (sizeof(T) == 2) {
         if (p.tile == 256) launch_layout<T, 256, 256, 2, 4, 2, 128, 2>(g, layout, grid, st);
+        else if (p.tile < p.tile_n) launch_layout<T, 64, 128, 2, 2, 2, 128, 2>(g, layout, grid, st);
     }
     if (p.tile == 128) launch_layout<T, 128, 128, 2, 2, 2, 128, 2>(g, layout, grid, st);
-    else if (p.tile == 64) launch_layout<T, 64, 64, 2, 2, 2, 128, 2>(g, layout, grid, st);
+    else if (p.tile_n == 64) launch_layout<T, 64, 64, 2, 2, 2, 128, 2>(g, layout, grid, st);
     if (p.splits > 1) {
         const int ppr = (g.N + 7) / 8;
         const long long pieces = (long long)g.M * ppr;

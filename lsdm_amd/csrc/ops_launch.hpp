@@ -9,7 +9,7 @@ namespace ops {
 
 constexpr int kNormMaxWidth = 16384;      // (1024 threads, 16 values each)
 
-struct GemmPlan { int tile = 0, tiles_m = 0, tiles_n = 0, splits = 1, kchunk = 0; };
+struct GemmPlan { int tile = 0, tile_n = 0, tiles_m = 0, tiles_n = 0, splits = 1, kchunk = 0; };
 
 struct PrepJob {
     const void* src = nullptr; long long lds = 0;

@@ -199,6 +199,17 @@ def test_linear_large_tiles(dt, M, K, N):
 
 
 @gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("M,K,N", [(2828, 2846, 2987), (5509, 666, 5667), (2089, 2099, 2028), (4762, 392, 2952), (1794, 1839, 1671), (1044, 1060, 2942)])
+def test_linear_every_tile(dt, M, K, N):
+    """Ragged sizes at which y, dx and dW are evaluated by the 256 x 256 tile (whole and split), the 128 x 128 one (whole; split) and the 64 x 128 one
+    (whole; dx split) in 16 bits, and by fp32's large tile."""
+    x, w, b, r, dy = linear_case(M, K, N, dt, 21, bias_f32=True)
+    y, g = run_linear(x, w, b, r, dy, "quick_gelu")
+    linear_check(x, w, b, r, dy, "quick_gelu", y, g)
+
+
+@gpu
 def test_linear_gradient_against_differences():
     gen = torch.Generator().manual_seed(3)
     x, w, b = (torch.randn(*s, generator=gen).to(DEV) for s in ((9, 12), (7, 12), (7,)))
