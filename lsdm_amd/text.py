@@ -57,8 +57,9 @@ def _dense_act(self, hidden_states):
 
 
 def _dense_residual_norm(self, hidden_states, input_tensor):
-    if self.training and self.dropout.p > 0:                       # the dropout sits between the product and the sum
-        return self.LayerNorm(self.dropout(self.dense(hidden_states)) + input_tensor)
+    drop = self.dropout                                            # it sits between the product and the sum, and its own mode says whether it drops
+    if type(drop) is not nn.Dropout or (drop.training and drop.p > 0):
+        return type(self).forward(self, hidden_states, input_tensor)
     return self.LayerNorm(self.dense(hidden_states, residual=input_tensor))
 
 
