@@ -10,12 +10,13 @@ of ``nn.Linear`` and ``nn.LayerNorm`` -- in place: parameters, names and ``state
 
 ``SceneDiffusionModel(..., text_kernels=True)`` does it for the tower the model loads itself.  What a block lets be fused is: BERT's
 ``dense -> activation`` and ``dense -> + input -> LayerNorm``, its pooler, and CLIP's ``x + c_proj(gelu(c_fc(ln_2(x))))``; everything else is replaced
-layer by layer, and attention itself stays with the package.  Autocast does not reach the operators: give the tower the type instead (a call that mixes
-types raises ``ValueError``).
+layer by layer, and attention itself stays with the package.  A block whose layers carry hooks runs unfused, so that they see what they always saw.
+Autocast does not reach the operators: give the tower the type instead (a call that mixes types raises ``ValueError``).
 """
 import functools
 
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import ops
 
@@ -52,22 +53,34 @@ class LayerNorm(nn.LayerNorm):
         return ops.layer_norm(x, self.weight, self.bias, self.eps, checkpoint8=self.checkpoint8)
 
 
+def _hooked(*modules):
+    """Whether someone looks at these layers' calls: a fused block leaves some of them out and gives others' results with more in them, so it runs its own
+    ``forward`` then."""
+    return _has_any_global_hook() or any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+
+
 def _dense_act(self, hidden_states):
+    if _hooked(self.dense, self.intermediate_act_fn):
+        return type(self).forward(self, hidden_states)
     return self.dense(hidden_states, self._kernel_activation)
 
 
 def _dense_residual_norm(self, hidden_states, input_tensor):
     drop = self.dropout                                            # it sits between the product and the sum, and its own mode says whether it drops
-    if type(drop) is not nn.Dropout or (drop.training and drop.p > 0):
+    if type(drop) is not nn.Dropout or (drop.training and drop.p > 0) or _hooked(self.dense, drop):
         return type(self).forward(self, hidden_states, input_tensor)
     return self.LayerNorm(self.dense(hidden_states, residual=input_tensor))
 
 
 def _pooler(self, hidden_states):
+    if _hooked(self.dense, self.activation):
+        return type(self).forward(self, hidden_states)
     return self.dense(hidden_states[:, 0], self._kernel_activation)
 
 
 def _clip_block(self, x):
+    if _hooked(self.mlp, *self.mlp):
+        return type(self).forward(self, x)
     x = x + self.attention(self.ln_1(x))
     return self.mlp.c_proj(self.mlp.c_fc(self.ln_2(x), self._kernel_activation), residual=x)
 

@@ -50,3 +50,83 @@ def test_dropout_layers_follow_their_own_mode():
         for seed in (5, 6):
             same(outputs(eager, ids(), seed), outputs(m, ids(), seed))
         assert torch.equal(outputs(m, ids(), 5), outputs(m, ids(), 6)) == tower_trains
+
+
+def _pairs():
+    """(eager, on the operators, the input) of both kinds of tower."""
+    x = torch.randn(5, 2, 64, generator=torch.Generator().manual_seed(4))
+    return [(towers.bert().eval(), towers.bert().eval(), ids()), (towers.clip_block().eval(), towers.clip_block().eval(), x)]
+
+
+def _hook_everything(m, into):
+    for name, layer in m.named_modules():
+        if name:
+            layer.register_forward_hook(lambda mod, args, out, name=name: into.append((name, (out[0] if isinstance(out, tuple) else out).detach())) if not hasattr(out, "keys") else None)
+
+
+@pytest.mark.parametrize("when", ["before", "after"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_hooks_fire_with_the_layers_own_values(which, when):
+    eager, m, x = _pairs()[which]
+    seen = [[], []]
+    _hook_everything(eager, seen[0])
+    if when == "before":
+        _hook_everything(m, seen[1])
+    use_kernels(m)
+    if when == "after":
+        _hook_everything(m, seen[1])
+    with torch.no_grad():
+        eager(x)
+        m(x)
+    assert [n for n, _ in seen[0]] == [n for n, _ in seen[1]]
+    for (_, a), (_, b) in zip(*seen):
+        same(a, b)
+
+
+HOOKED = [(0, "encoder.layer.0.intermediate.dense"), (0, "encoder.layer.0.intermediate.intermediate_act_fn"), (0, "encoder.layer.1.output.dense"),
+          (0, "encoder.layer.1.output.dropout"), (0, "encoder.layer.0.attention.output.dense"), (0, "pooler.dense"), (0, "pooler.activation"), (1, "mlp"), (1, "mlp.c_fc"),
+          (1, "mlp.gelu"), (1, "mlp.c_proj")]
+
+
+@pytest.mark.parametrize("kind", ["register_forward_pre_hook", "register_forward_hook", "register_full_backward_pre_hook", "register_full_backward_hook"])
+@pytest.mark.parametrize("which,name", HOOKED)
+def test_every_kind_of_hook_on_one_layer(which, name, kind):
+    """A hook on a single layer of a fused block, and its results once it is removed again."""
+    eager, m, x = _pairs()[which]
+    use_kernels(m)
+    seen = [[], []]
+    flat = lambda v: [t.detach() for t in v if isinstance(t, torch.Tensor)] if isinstance(v, tuple) else [v.detach()]
+    handles = [getattr(t.get_submodule(name), kind)(lambda mod, *vs, into=into: into.append([flat(v) for v in vs])) for t, into in zip((eager, m), seen)]
+    y = [t(x) for t in (eager, m)]
+    for v in y:
+        (v if which else v.pooler_output).square().sum().backward()
+    assert len(seen[0]) == len(seen[1]) == 1
+    for a, b in zip(seen[0][0], seen[1][0]):
+        assert len(a) == len(b)
+        for u, v in zip(a, b):
+            assert torch.allclose(u, v, rtol=1e-4, atol=1e-5)
+    for h in handles:
+        h.remove()
+    with torch.no_grad():
+        a, b = eager(x), m(x)
+        same(a if which else a.pooler_output, b if which else b.pooler_output)
+    assert len(seen[1]) == 1
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_hooks_on_every_module_of_the_process(which):
+    from torch.nn.modules.module import register_module_forward_hook
+    eager, m, x = _pairs()[which]
+    use_kernels(m)
+    names = [{id(v): n for n, v in t.named_modules()} for t in (eager, m)]
+    calls = []
+    handle = register_module_forward_hook(lambda mod, args, out: calls.append(id(mod)))
+    try:
+        with torch.no_grad():
+            eager(x)
+            first = [names[0][i] for i in calls]
+            calls.clear()
+            m(x)
+            assert [names[1][i] for i in calls] == first
+    finally:
+        handle.remove()
