@@ -10,7 +10,7 @@ of ``nn.Linear`` and ``nn.LayerNorm`` -- in place: parameters, names and ``state
 
 ``SceneDiffusionModel(..., text_kernels=True)`` does it for the tower the model loads itself.  What a block lets be fused is: BERT's
 ``dense -> activation`` and ``dense -> + input -> LayerNorm``, its pooler, and CLIP's ``x + c_proj(gelu(c_fc(ln_2(x))))``; everything else is replaced
-layer by layer, and attention itself stays with the package.  A block whose layers carry hooks runs unfused, so that they see what they always saw.
+layer by layer, and attention itself stays with the package.  A block whose layers carry hooks or were exchanged since runs its own ``forward``.
 Autocast does not reach the operators: give the tower the type instead (a call that mixes types raises ``ValueError``).
 """
 import functools
@@ -53,42 +53,58 @@ class LayerNorm(nn.LayerNorm):
         return ops.layer_norm(x, self.weight, self.bias, self.eps, checkpoint8=self.checkpoint8)
 
 
-def _hooked(*modules):
-    """Whether someone looks at these layers' calls: a fused block leaves some of them out and gives others' results with more in them, so it runs its own
-    ``forward`` then."""
-    return _has_any_global_hook() or any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+def _plain(*modules):
+    """Whether nobody looks at or changes these layers' calls (hooks, a ``forward`` put into the module): a fused block leaves some of them out and gives
+    others' results with more in them, so it runs its own ``forward`` where this is false."""
+    return not (_has_any_global_hook() or any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or "forward" in vars(m) for m in modules))
 
 
+# The fused forms ask at every call whether the block still holds what was fused: layers are exchanged (adapters, quantised layers) and hooked at any time.
 def _dense_act(self, hidden_states):
-    if _hooked(self.dense, self.intermediate_act_fn):
+    dense, act = self.dense, self.intermediate_act_fn
+    if type(dense) is not Linear or _activation_name(act) != self._kernel_activation or not _plain(dense, act):
         return type(self).forward(self, hidden_states)
-    return self.dense(hidden_states, self._kernel_activation)
+    return dense(hidden_states, self._kernel_activation)
 
 
 def _dense_residual_norm(self, hidden_states, input_tensor):
-    drop = self.dropout                                            # it sits between the product and the sum, and its own mode says whether it drops
-    if type(drop) is not nn.Dropout or (drop.training and drop.p > 0) or _hooked(self.dense, drop):
+    dense, drop = self.dense, self.dropout                         # the dropout sits between the product and the sum, and its own mode says whether it drops
+    if type(dense) is not Linear or type(drop) is not nn.Dropout or (drop.training and drop.p > 0) or not _plain(dense, drop):
         return type(self).forward(self, hidden_states, input_tensor)
-    return self.LayerNorm(self.dense(hidden_states, residual=input_tensor))
+    return self.LayerNorm(dense(hidden_states, residual=input_tensor))
 
 
 def _pooler(self, hidden_states):
-    if _hooked(self.dense, self.activation):
+    dense, act = self.dense, self.activation
+    if type(dense) is not Linear or _activation_name(act) != self._kernel_activation or not _plain(dense, act):
         return type(self).forward(self, hidden_states)
-    return self.dense(hidden_states[:, 0], self._kernel_activation)
+    return dense(hidden_states[:, 0], self._kernel_activation)
+
+
+_MLP = ["c_fc", "gelu", "c_proj"]
 
 
 def _clip_block(self, x):
-    if _hooked(self.mlp, *self.mlp):
+    mlp = self.mlp
+    layers = [*mlp._modules.values()]
+    if (type(mlp) is not nn.Sequential or [*mlp._modules] != _MLP or type(layers[0]) is not Linear or type(layers[2]) is not Linear
+            or _activation_name(layers[1]) != self._kernel_activation or not _plain(mlp, *layers)):
         return type(self).forward(self, x)
     x = x + self.attention(self.ln_1(x))
-    return self.mlp.c_proj(self.mlp.c_fc(self.ln_2(x), self._kernel_activation), residual=x)
+    return layers[2](layers[0](self.ln_2(x), self._kernel_activation), residual=x)
+
+
+_FUSED = (_dense_act, _dense_residual_norm, _pooler, _clip_block)
 
 
 def _fuse(module):
     """Replaces the ``forward`` of a block whose layers form one of the fused patterns: exactly these children, the dense layers among them replaced above (a
-    subclass of ``nn.Linear``, or a further layer in the block, keeps the block's own ``forward``)."""
-    name, children = type(module).__name__, dict(module.named_children())
+    subclass of ``nn.Linear``, a further layer in the block, or a ``forward`` that someone put into the module keeps the block as it is)."""
+    name, children, own = type(module).__name__, dict(module.named_children()), vars(module).get("forward")
+    if isinstance(own, functools.partial) and own.func in _FUSED:
+        del module.forward                                         # an earlier call's: the block may have changed since
+    elif own is not None:
+        return
     mlp = dict(children["mlp"].named_children()) if "mlp" in children else {}
     if set(children) != _BLOCKS.get(name) or any(type(c) is not Linear for n, c in [*children.items(), *mlp.items()] if n in _DENSE):
         return
@@ -99,7 +115,7 @@ def _fuse(module):
         act, forward = "none", _dense_residual_norm
     elif name == "BertPooler":
         act, forward = _activation_name(module.activation), _pooler
-    elif name == "ResidualAttentionBlock" and hasattr(module, "attention") and list(mlp) == ["c_fc", "gelu", "c_proj"]:
+    elif name == "ResidualAttentionBlock" and hasattr(module, "attention") and list(mlp) == _MLP:
         act, forward = _activation_name(module.mlp.gelu), _clip_block
     else:
         return

@@ -130,3 +130,67 @@ def test_hooks_on_every_module_of_the_process(which):
             assert [names[1][i] for i in calls] == first
     finally:
         handle.remove()
+
+
+class Adapter(torch.nn.Module):
+    """A layer a user puts around a dense one."""
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x):
+        return self.inner(x) + 0.5 * x.mean(-1, keepdim=True)
+
+
+def _adapt(m, name, change):
+    block, child = m.get_submodule(name.rpartition(".")[0]) if "." in name else m, name.rpartition(".")[2]
+    setattr(block, child, change(getattr(block, child)))
+
+
+CHANGES = [(0, "encoder.layer.0.intermediate.dense", Adapter), (0, "encoder.layer.1.output.dense", Adapter), (0, "pooler.dense", Adapter),
+           (0, "encoder.layer.0.intermediate.intermediate_act_fn", lambda old: torch.nn.ReLU()), (0, "encoder.layer.0.intermediate.intermediate_act_fn", lambda old: torch.nn.Softplus()),
+           (0, "pooler.activation", lambda old: torch.nn.GELU(approximate="tanh")), (0, "encoder.layer.1.output.dropout", Adapter),
+           (1, "mlp.c_fc", Adapter), (1, "mlp.c_proj", Adapter), (1, "mlp.gelu", lambda old: torch.nn.SiLU()),
+           (1, "mlp", lambda old: torch.nn.Sequential(*old, torch.nn.Tanh())), (1, "mlp", Adapter)]
+
+
+@pytest.mark.parametrize("again", [False, True])
+@pytest.mark.parametrize("i", range(len(CHANGES)), ids=["%s-%d" % (c[1], i) for i, c in enumerate(CHANGES)])
+def test_layers_exchanged_after_use_kernels(i, again):
+    which, name, change = CHANGES[i]
+    eager, m, x = _pairs()[which]
+    use_kernels(m)
+    for t in (eager, m):
+        _adapt(t, name, change)
+    if again:
+        use_kernels(m)
+    with torch.no_grad():
+        a, b = eager(x), m(x)
+    same(a if which else a.last_hidden_state, b if which else b.last_hidden_state)
+    if not which:
+        same(a.pooler_output, b.pooler_output)
+
+
+@pytest.mark.parametrize("name", ["encoder.layer.0.intermediate", "encoder.layer.1.output", "pooler"])
+def test_a_blocks_own_forward_is_kept(name):
+    """Packages that place a module's calls put a function of their own into the module as ``forward``."""
+    m, calls = towers.bert().eval(), []
+    block = m.get_submodule(name)
+    inner = block.forward
+    block.forward = lambda *a: calls.append(name) or inner(*a)
+    kept = block.forward
+    use_kernels(m)
+    use_kernels(m)
+    assert block.forward is kept
+    with torch.no_grad():
+        same(m(ids()).pooler_output, towers.bert().eval()(ids()).pooler_output)
+    assert calls == [name]
+
+
+def test_layers_with_a_forward_of_their_own_inside_a_block():
+    eager, m, x = _pairs()[1]
+    use_kernels(m)
+    for t in (eager, m):
+        t.mlp.gelu.forward = lambda z: z.clamp(min=0)
+    with torch.no_grad():
+        same(eager(x), m(x))
