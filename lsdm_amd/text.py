@@ -97,12 +97,25 @@ def _clip_block(self, x):
 _FUSED = (_dense_act, _dense_residual_norm, _pooler, _clip_block)
 
 
+def _put(module, forward):
+    module.forward = functools.partial(forward, module)           # (copies and pickles with the module, as a bound method would not)
+    module._replicate_for_data_parallel = functools.partial(_replicate, module)
+
+
+def _replicate(module):
+    """A replica's attributes are copied one by one, the module inside ``forward`` would stay the original."""
+    replica = type(module)._replicate_for_data_parallel(module)
+    _put(replica, module.forward.func)
+    return replica
+
+
 def _fuse(module):
     """Replaces the ``forward`` of a block whose layers form one of the fused patterns: exactly these children, the dense layers among them replaced above (a
     subclass of ``nn.Linear``, a further layer in the block, or a ``forward`` that someone put into the module keeps the block as it is)."""
     name, children, own = type(module).__name__, dict(module.named_children()), vars(module).get("forward")
     if isinstance(own, functools.partial) and own.func in _FUSED:
-        del module.forward                                         # an earlier call's: the block may have changed since
+        for attribute in ("forward", "_replicate_for_data_parallel"):     # an earlier call's: the block may have changed since
+            vars(module).pop(attribute, None)
     elif own is not None:
         return
     mlp = dict(children["mlp"].named_children()) if "mlp" in children else {}
@@ -121,7 +134,7 @@ def _fuse(module):
         return
     if act is not None:
         module._kernel_activation = act
-        module.forward = functools.partial(forward, module)       # (copies and pickles with the module, as a bound method would not)
+        _put(module, forward)
 
 
 def use_kernels(tower, *, checkpoint8=False):

@@ -194,3 +194,26 @@ def test_layers_with_a_forward_of_their_own_inside_a_block():
         t.mlp.gelu.forward = lambda z: z.clamp(min=0)
     with torch.no_grad():
         same(eager(x), m(x))
+
+
+@pytest.mark.parametrize("which,name", [(0, "encoder.layer.0.intermediate"), (0, "encoder.layer.1.output"), (0, "pooler"), (1, "")])
+def test_replicas_call_their_own_layers(which, name):
+    """What torch.nn.parallel.replicate does to a module: a copy of its attributes, whose children and parameters are then exchanged."""
+    _, m, x = _pairs()[which]
+    use_kernels(m)
+    block = m.get_submodule(name)
+    torch.manual_seed(9)
+    args = [torch.randn(4, 3, 200 if name.endswith("output") else 64 if which else 96)] + [torch.randn(4, 3, 96)] * name.endswith("output")
+    with torch.no_grad():
+        before = block(*args)
+        other = block._replicate_for_data_parallel()._replicate_for_data_parallel()
+        for child in ("mlp",) if which else ("dense",):
+            old = getattr(other, child)
+            new = use_kernels(towers.clip_block()).mlp if which else type(old)(old.in_features, old.out_features)
+            for p in new.parameters():
+                p.normal_()
+            other._modules = dict(other._modules)
+            other._modules[child] = new
+        after = other(*args)
+        assert torch.equal(block(*args), before) and not torch.allclose(after, before, atol=1e-2)
+        same(after, type(other).forward(other, *args))
