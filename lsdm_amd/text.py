@@ -14,6 +14,7 @@ layer by layer, and attention itself stays with the package.  A block whose laye
 Autocast does not reach the operators: give the tower the type instead (a call that mixes types raises ``ValueError``).
 """
 import functools
+import inspect
 
 import torch.nn as nn
 from torch.nn.modules.module import _has_any_global_hook
@@ -25,7 +26,7 @@ _ACT_BY_CLASS = {"GELUActivation": "gelu", "GELU": "gelu", "QuickGELU": "quick_g
                  "ReLU": "relu", "Sigmoid": "sigmoid", "Tanh": "tanh"}
 
 
-# the blocks that are fused, by class and children
+# the blocks that are fused, by class and children: BERT's of ``transformers``; CLIP's of any package that carries it, known by its ``forward(x)`` as well
 _BLOCKS = {"BertIntermediate": {"dense", "intermediate_act_fn"}, "BertSelfOutput": {"dense", "LayerNorm", "dropout"}, "BertOutput": {"dense", "LayerNorm", "dropout"},
            "BertPooler": {"dense", "activation"}, "ResidualAttentionBlock": {"attn", "ln_1", "mlp", "ln_2"}}
 _DENSE = ("dense", "c_fc", "c_proj")
@@ -119,6 +120,11 @@ def _fuse(module):
     elif own is not None:
         return
     mlp = dict(children["mlp"].named_children()) if "mlp" in children else {}
+    if name == "ResidualAttentionBlock":
+        if list(inspect.signature(type(module).forward).parameters) != ["self", "x"]:
+            return
+    elif type(module).__module__.split(".")[0] != "transformers":
+        return
     if set(children) != _BLOCKS.get(name) or any(type(c) is not Linear for n, c in [*children.items(), *mlp.items()] if n in _DENSE):
         return
     if name == "BertIntermediate":

@@ -217,3 +217,31 @@ def test_replicas_call_their_own_layers(which, name):
         after = other(*args)
         assert torch.equal(block(*args), before) and not torch.allclose(after, before, atol=1e-2)
         same(after, type(other).forward(other, *args))
+
+
+class BertOutput(torch.nn.Module):
+    """Not the package's: the same name and layers in another order."""
+    def __init__(self):
+        super().__init__()
+        self.dense, self.LayerNorm, self.dropout = torch.nn.Linear(24, 24), torch.nn.LayerNorm(24), torch.nn.Dropout(0.0)
+
+    def forward(self, hidden_states, input_tensor):
+        return self.dropout(self.dense(self.LayerNorm(hidden_states))) + input_tensor
+
+
+def test_blocks_of_other_packages_keep_their_forward():
+    a, b = torch.randn(2, 5, 24)
+    torch.manual_seed(3)
+    eager = BertOutput()
+    torch.manual_seed(3)
+    m = use_kernels(BertOutput())
+    with torch.no_grad():
+        same(eager(a, b), m(a, b))
+    # CLIP's block is known by its structure (several packages carry it): one whose forward takes more is not it
+    block = towers.clip_block()
+    type(block).forward = lambda self, x, mask=None: x + self.mlp(self.ln_2(x))
+    x = torch.randn(5, 2, 64)
+    with torch.no_grad():
+        want = block(x)
+        same(use_kernels(block)(x), want)
+        same(block(x, mask=None), want)
