@@ -23,8 +23,11 @@ would show: in float32 ``linear`` keeps a'(z) in 32 bits, and ``layer_norm`` ref
 HIP graphs: forward and backward passes can be captured.  A leaf whose gradient node is held by a live autograd graph built eagerly on the default
 stream cannot take part in a capture (the runtime would have to join the default stream to it): such a call raises ``LsdmError``.
 """
+import torch
+
 from . import _lib
 
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "quick_gelu": 3, "silu": 4, "sigmoid": 5, "tanh": 6}
 NORM_MAX_WIDTH = 16384
 

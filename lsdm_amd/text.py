@@ -143,24 +143,28 @@ def _fuse(module):
         _put(module, forward)
 
 
+def _layer_class(module):
+    """The class that takes ``module``'s place, or None."""
+    kind = type(module)
+    if kind in (nn.Linear, Linear):
+        return Linear
+    if kind in (nn.LayerNorm, LayerNorm) or (isinstance(module, nn.LayerNorm) and kind.__module__.split(".")[0] == "clip"):
+        return LayerNorm if len(module.normalized_shape) == 1 and module.normalized_shape[0] <= ops.NORM_MAX_WIDTH else None
+    return None
+
+
 def use_kernels(tower, *, checkpoint8=False):
-    """Puts the operators under ``tower``'s layers, in place; returns ``tower``.  Layers of other kinds are left as they are.  Raises ``ValueError`` if
-    there is nothing to replace."""
-    found = 0
-    for module in tower.modules():
-        kind = type(module)
-        if kind in (nn.Linear, Linear):
-            module.__class__ = Linear
-        elif kind in (nn.LayerNorm, LayerNorm) or (isinstance(module, nn.LayerNorm) and kind.__module__.split(".")[0] == "clip"):
-            if len(module.normalized_shape) != 1 or module.normalized_shape[0] > ops.NORM_MAX_WIDTH:
-                continue
-            module.__class__ = LayerNorm
-        else:
-            continue
-        module.checkpoint8 = checkpoint8
-        found += 1
+    """Puts the operators under ``tower``'s layers, in place; returns ``tower``.  Layers of other kinds are left as they are.  Raises ``ValueError``, and
+    changes nothing, if there is nothing to replace or a layer's parameters have a type that the operators do not take (float64)."""
+    found = [(module, _layer_class(module)) for module in tower.modules() if _layer_class(module)]
     if not found:
         raise ValueError("use_kernels: no Linear or LayerNorm layer in %s" % type(tower).__name__)
+    for module, kind in found:
+        if module.weight is not None and module.weight.dtype not in ops.DTYPES:
+            raise ValueError("use_kernels: a %s layer holds %s parameters; the operators take float32, bfloat16 and float16" % (kind.__name__, module.weight.dtype))
+    for module, kind in found:
+        module.__class__ = kind
+        module.checkpoint8 = checkpoint8
     for module in tower.modules():
         _fuse(module)
     return tower

@@ -245,3 +245,16 @@ def test_blocks_of_other_packages_keep_their_forward():
         want = block(x)
         same(use_kernels(block)(x), want)
         same(block(x, mask=None), want)
+
+
+def test_a_tower_of_a_type_without_kernels_is_refused_as_a_whole():
+    m = towers.bert().double()
+    kinds = [type(v) for v in m.modules()]
+    with pytest.raises(ValueError, match="float64"):
+        use_kernels(m)
+    assert [type(v) for v in m.modules()] == kinds and not any("forward" in vars(v) for v in m.modules())
+    mixed = torch.nn.Sequential(torch.nn.Linear(4, 4), torch.nn.LayerNorm(4, dtype=torch.float64))
+    with pytest.raises(ValueError, match="float64"):
+        use_kernels(mixed)
+    assert type(mixed[0]) is torch.nn.Linear
+    assert use_kernels(torch.nn.Sequential(torch.nn.Linear(4, 4), torch.nn.LayerNorm(4, elementwise_affine=False))) is not None
