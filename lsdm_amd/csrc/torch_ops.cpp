@@ -3,6 +3,8 @@
 // a forward and backward pass whose kernels take 20.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/lsdm_hip.h"
@@ -43,6 +45,16 @@ int dtype_of(at::ScalarType t) {
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// A tracer (torch.jit.trace, make_fx, fake tensors) records tensors' operations; what the kernels write through pointers is none, and the recorded graph would
+// return memory that nothing wrote.
+void check_traced(const char* who) {
+    using c10::impl::TorchDispatchModeKey;
+    bool traced = torch::jit::tracer::isTracing();
+    if (c10::impl::TorchDispatchModeTLS::any_modes_set())
+        for (const auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+            traced = traced || c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
+    if (traced) throw LsdmFailure(text(who, " cannot be traced: its kernels run outside of torch's operations (capture the call into a HIP graph instead)"));
+}
 void check_operand(const char* who, const Tensor& x) {
     if (!x.is_cuda()) throw LsdmFailure(text(who, " runs in liblsdm_hip.so on HIP device tensors; got ", x.device()));
     if (x.layout() != at::kStrided || dtype_of(x.scalar_type()) < 0) value_error(who, ": a dense tensor of dtype float32, bfloat16 or float16 is needed, got ", x.scalar_type());
@@ -109,6 +121,7 @@ std::pair<Tensor, Tensor> pack_rows(const Rows& x, int64_t width) {
 }
 
 std::pair<Tensor, Tensor> pack8(const Tensor& x_) {
+    check_traced("checkpoint8");
     check_operand("checkpoint8", x_);
     const Tensor x = x_.detach();
     if (x.dim() < 1) value_error("checkpoint8: a tensor of at least one axis is needed");
@@ -120,6 +133,7 @@ std::pair<Tensor, Tensor> pack8(const Tensor& x_) {
 }
 
 Tensor unpack8(const Tensor& codes, const Tensor& exps, const std::vector<int64_t>& shape, at::ScalarType dtype) {
+    check_traced("Checkpoint8.restore");
     if (dtype_of(dtype) < 0) value_error("Checkpoint8.restore: dtype must be float32, bfloat16 or float16, got ", dtype);
     if (!codes.is_cuda() || exps.device() != codes.device()) throw LsdmFailure("Checkpoint8.restore: codes and exps must be on one HIP device");
     const bool dense = codes.dim() == 2 && codes.scalar_type() == at::kChar && codes.is_contiguous() && exps.dim() == 2 && exps.scalar_type() == at::kByte &&
@@ -175,6 +189,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         return f.y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_traced("the backward pass of linear");
         const Tensor& dy_ = grads[0];
         variable_list out(9);
         if (!dy_.defined()) return out;
@@ -229,6 +244,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 
 Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias_, int64_t act, const std::optional<Tensor>& residual_, bool checkpoint) {
     const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+    check_traced("linear");
     check_operand("linear", x);
     check_device("linear", "weight", w, x);
     check_device("linear", "bias", bias, x);
@@ -292,6 +308,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         return f.y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_traced("the backward pass of layer_norm");
         const Tensor& dy_ = grads[0];
         variable_list out(5);
         if (!dy_.defined()) return out;
@@ -323,6 +340,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& w_, const std::optional<Tensor>& b_, double eps, bool checkpoint) {
     const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
+    check_traced("layer_norm");
     check_operand("layer_norm", x);
     check_device("layer_norm", "weight", w, x);
     check_device("layer_norm", "bias", b, x);

@@ -20,6 +20,7 @@ is never hidden.  ``linear(..., checkpoint8=True)`` keeps ``x`` in this form and
 ``layer_norm(..., checkpoint8=True)`` keeps the normalised rows.  Codes taken from computed values flip on their last bit, which float32 gradients
 would show: in float32 ``linear`` keeps a'(z) in 32 bits, and ``layer_norm`` refuses ``checkpoint8``.
 
+Tracers (``torch.jit.trace``, ``make_fx``, fake tensors) do not see what the kernels write: such calls raise ``LsdmError``.
 HIP graphs: forward and backward passes can be captured.  A leaf whose gradient node is held by a live autograd graph built eagerly on the default
 stream cannot take part in a capture (the runtime would have to join the default stream to it): such a call raises ``LsdmError``.
 """

@@ -1,0 +1,57 @@
+"""How the public operators are called: under a tracer."""
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from lsdm_amd import _lib, ops
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(autouse=True)
+def _grad_mode():
+    with torch.enable_grad():
+        yield
+
+
+def calls(device):
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen).to(device)
+    x, w, b, res, n = r(70, 16), r(8, 16), r(8), r(70, 8), r(16)
+    return x, [lambda t: ops.linear(t, w), lambda t: ops.linear(x, w, b, "gelu", residual=t @ w.t()), lambda t: ops.linear(res, t[:, :8].contiguous()),
+               lambda t: ops.layer_norm(t), lambda t: ops.layer_norm(x, t[0].contiguous(), n)]
+
+
+def refuse_tracing(device):
+    x, forms = calls(device)
+    packed = lambda t: ops.checkpoint8(t).codes
+    for f in [*forms, packed]:
+        with pytest.raises(_lib.LsdmError, match="traced"):
+            torch.jit.trace(f, (x,))
+        with pytest.raises(_lib.LsdmError, match="traced"):
+            make_fx(f)(x)
+
+
+def test_traced_calls_are_refused_on_the_host():
+    refuse_tracing("cpu")
+
+
+@gpu
+def test_traced_calls_are_refused():
+    """A tracer records tensors' operations, and these kernels write through pointers: the recorded graph would return memory that nothing wrote."""
+    refuse_tracing(DEV)
+    c = ops.checkpoint8(torch.randn(3, 40, device=DEV))
+    with pytest.raises(_lib.LsdmError, match="traced"):
+        torch.jit.trace(lambda t: ops.Checkpoint8(t, c.exps, c.shape, c.dtype).restore(), (c.codes,))
+    x, forms = calls(DEV)
+    for f in forms:
+        assert torch.equal(f(x), f(x))                      # and are what they were afterwards
+    t = x.clone().requires_grad_(True)
+    for f in (forms[0], forms[3]):
+        y = f(t)
+        dy = torch.randn_like(y)
+        want = torch.autograd.grad(y, [t], dy, retain_graph=True)[0]
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda g: torch.autograd.grad(y, [t], g, retain_graph=True)[0])(dy)
+        assert torch.equal(torch.autograd.grad(y, [t], dy)[0], want)
