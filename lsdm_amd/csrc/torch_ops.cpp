@@ -55,6 +55,11 @@ void check_traced(const char* who) {
             traced = traced || c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
     if (traced) throw LsdmFailure(text(who, " cannot be traced: its kernels run outside of torch's operations (capture the call into a HIP graph instead)"));
 }
+// a dual tensor's tangent would be dropped, which reads as a derivative of zero
+void check_tangents(const char* who, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->_fw_grad(0).defined()) throw LsdmFailure(text(who, " has no forward-mode derivative; an input carries a tangent"));
+}
 void check_operand(const char* who, const Tensor& x) {
     if (!x.is_cuda()) throw LsdmFailure(text(who, " runs in liblsdm_hip.so on HIP device tensors; got ", x.device()));
     if (x.layout() != at::kStrided || dtype_of(x.scalar_type()) < 0) value_error(who, ": a dense tensor of dtype float32, bfloat16 or float16 is needed, got ", x.scalar_type());
@@ -245,6 +250,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias_, int64_t act, const std::optional<Tensor>& residual_, bool checkpoint) {
     const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
     check_traced("linear");
+    check_tangents("linear", {&x, &w, &bias, &residual});
     check_operand("linear", x);
     check_device("linear", "weight", w, x);
     check_device("linear", "bias", bias, x);
@@ -341,6 +347,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& w_, const std::optional<Tensor>& b_, double eps, bool checkpoint) {
     const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
     check_traced("layer_norm");
+    check_tangents("layer_norm", {&x, &w, &b});
     check_operand("layer_norm", x);
     check_device("layer_norm", "weight", w, x);
     check_device("layer_norm", "bias", b, x);

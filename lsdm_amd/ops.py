@@ -12,7 +12,7 @@ Types: float32, bfloat16, float16, the same for all tensors of a call (``bias`` 
 accumulate and everything else is evaluated in 32 bits; results are rounded once.  In 16 bits the backward pass of ``linear`` rounds dz = dy a'(z) to the
 tensors' type, as the matrix cores take their operands in it (a'(z) itself is kept with 13 significant bits).
 Shapes: any leading axes, any sizes including 0 rows (at most 2^30 rows and columns, 2^25 rows of ``weight``, 2^35 values of a checkpoint); the last axis should be contiguous (other layouts are copied first).
-Gradients are differentiable once.  Results do not depend on timing (no atomics): the same call gives the same bits.
+Gradients are differentiable once; forward-mode derivatives there are none (a dual tensor raises ``LsdmError``).  Results do not depend on timing (no atomics): the same call gives the same bits.
 
 8-bit checkpoints: groups of 32 consecutive values of a row share a power-of-two step 2^e (e = max(floor(log2 max|x|) - 6, -126)); a value is kept
 as the int8 nearest to x / 2^e.  What is restored is exact in every type; a group that holds an infinity or a NaN comes back as NaN, so an overflow

@@ -1,6 +1,7 @@
-"""How the public operators are called: under a tracer."""
+"""How the public operators are called: under a tracer, with forward-mode derivatives."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from lsdm_amd import _lib, ops
@@ -33,6 +34,15 @@ def refuse_tracing(device):
             make_fx(f)(x)
 
 
+def refuse_forward_mode(device):
+    x, forms = calls(device)
+    for f in forms:
+        with forward_ad.dual_level():
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(_lib.LsdmError, match="forward-mode"):
+                    f(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
 def test_traced_calls_are_refused_on_the_host():
     refuse_tracing("cpu")
 
@@ -55,3 +65,17 @@ def test_traced_calls_are_refused():
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(lambda g: torch.autograd.grad(y, [t], g, retain_graph=True)[0])(dy)
         assert torch.equal(torch.autograd.grad(y, [t], dy)[0], want)
+
+
+def test_forward_mode_is_refused_on_the_host():
+    refuse_forward_mode("cpu")
+
+
+@gpu
+def test_forward_mode_is_refused():
+    refuse_forward_mode(DEV)
+    x, forms = calls(DEV)
+    with forward_ad.dual_level():
+        for f in forms:                                     # a dual number elsewhere does not matter
+            d = forward_ad.make_dual(torch.ones(3, device=DEV), torch.ones(3, device=DEV))
+            assert torch.equal(f(x), f(x)) and forward_ad.unpack_dual(d).tangent is not None
