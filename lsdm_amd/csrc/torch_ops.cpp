@@ -9,6 +9,8 @@
 
 #include "../../include/lsdm_hip.h"
 
+#include <unordered_set>
+
 namespace {
 
 using at::Tensor;
@@ -84,8 +86,9 @@ bool unaligned(const Rows& r, int64_t width) {
 Tensor scratch(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 Tensor maybe_contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 
-// A leaf whose gradient node is alive and sits on the default stream cannot take part in a capture on another stream: autograd would have to join
-// the default stream to it, and the failure surfaces where the process cannot recover.  Refused before anything is recorded.
+// A graph node that sits on the default stream -- a leaf's gradient node that an eager graph keeps alive, or a part of such a graph -- cannot take part in a
+// capture on another stream: autograd would have to join the default stream to it, and the failure surfaces where the process cannot recover.  Everything
+// that the call's backward pass can reach is looked at (a leaf may stand behind casts and views), and the call refused before anything is recorded.
 void check_capture(const char* who, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
     const auto current = c10::hip::getCurrentHIPStream(x.device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -94,15 +97,23 @@ void check_capture(const char* who, const Tensor& x, std::initializer_list<const
         return;
     }
     if (status == hipStreamCaptureStatusNone) return;
-    for (const Tensor* t : inputs) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (!node) continue;
+    const auto def = c10::hip::getDefaultHIPStream(x.device().index());
+    std::vector<std::shared_ptr<torch::autograd::Node>> open;
+    std::unordered_set<torch::autograd::Node*> seen;
+    auto visit = [&](const std::shared_ptr<torch::autograd::Node>& n) {
+        if (n && seen.insert(n.get()).second) open.push_back(n);
+    };
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->requires_grad()) visit(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!open.empty()) {
+        const auto node = std::move(open.back());
+        open.pop_back();
         const auto s = node->stream();
         // (by number: the node's stream carries the device type that torch shows, this one the runtime's)
-        if (s && s->device_index() == x.device().index() && s->id() != current.id() && s->id() == c10::hip::getDefaultHIPStream(x.device().index()).id())
-            throw LsdmFailure(text(who, ": a leaf of this captured call is held by a live autograd graph that was built on the default stream; release that graph "
-                                        "(or build it on a side stream) before the capture"));
+        if (s && s->device_index() == x.device().index() && s->id() != current.id() && s->id() == def.id())
+            throw LsdmFailure(text(who, ": a leaf of this captured call, or a part of the graph behind it, is held by a live autograd graph that was built on the default "
+                                        "stream; release that graph (or build it on a side stream) before the capture"));
+        for (const auto& e : node->next_edges()) visit(e.function);
     }
 }
 

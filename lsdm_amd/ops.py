@@ -22,7 +22,8 @@ would show: in float32 ``linear`` keeps a'(z) in 32 bits, and ``layer_norm`` ref
 
 Tracers (``torch.jit.trace``, ``make_fx``, fake tensors) do not see what the kernels write: such calls raise ``LsdmError``.
 HIP graphs: forward and backward passes can be captured.  A leaf whose gradient node is held by a live autograd graph built eagerly on the default
-stream cannot take part in a capture (the runtime would have to join the default stream to it): such a call raises ``LsdmError``.
+stream cannot take part in a capture (the runtime would have to join the default stream to it), whether it is an input itself or stands behind one: such a
+call raises ``LsdmError``.
 """
 import torch
 

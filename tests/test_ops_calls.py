@@ -1,4 +1,4 @@
-"""How the public operators are called: under a tracer, with forward-mode derivatives."""
+"""How the public operators are called: under a tracer, with forward-mode derivatives, while a graph is captured."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -79,3 +79,37 @@ def test_forward_mode_is_refused():
         for f in forms:                                     # a dual number elsewhere does not matter
             d = forward_ad.make_dual(torch.ones(3, device=DEV), torch.ones(3, device=DEV))
             assert torch.equal(f(x), f(x)) and forward_ad.unpack_dual(d).tangent is not None
+
+
+@gpu
+def test_capture_with_a_live_eager_graph_behind_the_inputs_is_refused():
+    """The captured call's inputs are not the leaves themselves but computed from them inside the capture (a cast, a slice, a tied weight): the backward
+    pass would end at the leaves' gradient nodes on the default stream all the same."""
+    w = torch.randn(8, 16, device=DEV, requires_grad=True)
+    n = torch.ones(16, device=DEV, requires_grad=True)
+    b = torch.zeros(8, device=DEV, requires_grad=True)
+    x = torch.randn(70, 16, device=DEV)
+    alive = [ops.linear(x, w, b), ops.layer_norm(x, n)]     # built on the default stream
+    own = torch.randn(8, 16, device=DEV, requires_grad=True)    # a leaf no eager graph holds
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    refused, taken = [], []
+    with torch.cuda.graph(g, stream=s):
+        for f in (lambda: ops.linear(x.half(), w.half()), lambda: ops.linear(x, w[:4]), lambda: ops.linear(x, w.detach(), b * 2), lambda: ops.layer_norm(x, n * 0.5),
+                  lambda: ops.layer_norm(ops.linear(x[:, :8].contiguous(), (w.t() + 1.0).contiguous())), lambda: ops.layer_norm((x + n).view(7, 10, 16))):
+            try:
+                f()
+            except _lib.LsdmError as e:
+                refused.append(str(e))
+        y = ops.linear(x.half(), own.half() * 2, w.detach()[:, 0])
+        taken += [y, *torch.autograd.grad(y, [own], torch.ones_like(y))]
+    assert len(refused) == 6 and all("live autograd graph" in r for r in refused)
+    y = ops.linear(x.half(), own.half() * 2, w.detach()[:, 0])
+    want = [y, *torch.autograd.grad(y, [own], torch.ones_like(y))]
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(taken, want))
+    torch.autograd.grad(alive[0], [w, b], torch.ones_like(alive[0]))      # the eager graphs are as they were
+    torch.autograd.grad(alive[1], [n], torch.ones_like(alive[1]))
