@@ -1,4 +1,6 @@
-"""How the public operators are called: under a tracer, with forward-mode derivatives, while a graph is captured."""
+"""How the public operators are called: under a tracer, with forward-mode derivatives, while a graph is captured, from several threads."""
+import threading
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -113,3 +115,38 @@ def test_capture_with_a_live_eager_graph_behind_the_inputs_is_refused():
         assert all(torch.equal(a, b) for a, b in zip(taken, want))
     torch.autograd.grad(alive[0], [w, b], torch.ones_like(alive[0]))      # the eager graphs are as they were
     torch.autograd.grad(alive[1], [n], torch.ones_like(alive[1]))
+
+
+@gpu
+def test_calls_from_several_threads():
+    """Every thread on a stream of its own, forward and backward, with refused calls in between: the results of one thread alone."""
+    gen = torch.Generator().manual_seed(1)
+    sets = []
+    for k in range(4):
+        r = lambda *s: torch.randn(*s, generator=gen).to(DEV).bfloat16()
+        sets.append([r(300 + 41 * k, 72), r(88, 72), r(88), r(300 + 41 * k, 88), r(88), r(300 + 41 * k, 88)])
+
+    def work(v):
+        x, w, b, res, n, dy = (t.clone().requires_grad_(True) for t in v)
+        y = ops.layer_norm(ops.linear(x, w, b, "silu", res), n)
+        return [y.detach(), *torch.autograd.grad(y, [x, w, b, res, n], dy.detach())]
+    want = [work(v) for v in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(k):
+        s = torch.cuda.Stream()
+        with torch.enable_grad(), torch.cuda.stream(s):
+            for i in range(6):
+                got = work(sets[k])
+                with pytest.raises(ValueError, match="eps"):
+                    ops.layer_norm(sets[k][0], eps=-1.0 - k)
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                    wrong.append((k, i))
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
