@@ -10,7 +10,9 @@
 // order by a second launch (no atomics: results do not depend on the schedule).
 // A row is read and written in pieces of eight elements (ops.hpp), whatever its width and alignment.
 // Measured, bf16 (a copy runs at 4.9 TB/s): 32768 x 2048 forward 44.5 us (6.0 TB/s), backward 76 us (5.3), with h in 8 bits 57 and 65 us; 4928 x 771
-// forward 7.0 us, backward 20; fp32 32768 x 2048 107 and 148 us.
+// forward 7.5 us, backward 20; fp32 32768 x 2048 107 and 148 us.
+#include <type_traits>
+
 #include "ops.hpp"
 #include "ops_launch.hpp"
 
@@ -40,11 +42,12 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <int W>
 __device__ __forceinline__ unsigned lanes_max(unsigned v) { return lanes_join<W>(v, [](unsigned a, unsigned b) { return max(a, b); }); }
 
-// both sums over the NT threads of a row; red: one entry per wave of the work-group
-template <int NT>
+// over the NT threads of a row: both sums, or the sum and (MAX) the largest of values >= 0; red: one entry per wave of the work-group
+template <int NT, bool MAX = false>
 __device__ __forceinline__ float2 row_sum2(float a, float b, float2* red, int t) {
-    a = lanes_sum<(NT < 64 ? NT : 64)>(a);
-    b = lanes_sum<(NT < 64 ? NT : 64)>(b);
+    constexpr int W = NT < 64 ? NT : 64;
+    a = lanes_sum<W>(a);
+    b = MAX ? __builtin_bit_cast(float, lanes_max<W>(__builtin_bit_cast(unsigned, b))) : lanes_sum<W>(b);
     if constexpr (NT > 64) {
         constexpr int NW = NT / 64;
         const int first = (t / NT) * NW;         // the row's waves
@@ -53,7 +56,7 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* red, int t)
         wg_sync();
         a = 0.0f; b = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) { a += red[first + i].x; b += red[first + i].y; }
+        for (int i = 0; i < NW; ++i) { a += red[first + i].x; b = MAX ? fmaxf(b, red[first + i].y) : b + red[first + i].y; }
     }
     return make_float2(a, b);
 }
@@ -156,6 +159,12 @@ __device__ __forceinline__ void param_load(const void* p, int is_f32, float miss
         for (int j = 0; j < 8; ++j) v[i][j] = missing;
 }
 
+// a / b, correctly rounded, from the rounded reciprocal of b
+__device__ __forceinline__ float over(float a, float b, float inv_b) {
+    const float q = a * inv_b;
+    return fmaf(fmaf(-q, b, a), inv_b, q);
+}
+
 template <class T, int NT, int NV, bool WHOLE>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_fwd_kernel(NormArgs a) {
     constexpr int THREADS = NT > 256 ? NT : 256, RPG = THREADS / NT;
@@ -164,7 +173,8 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_fwd_kernel(NormArgs 
     float w[NV][8], b[NV][8];
     param_load<T, NT, NV, WHOLE>(a.w, a.param_f32, 1.0f, D, l, w);
     param_load<T, NT, NV, WHOLE>(a.b, a.param_f32, 0.0f, D, l, b);
-    const float inv_d = 1.0f / (float)D;
+    constexpr bool SCALED = !std::is_same<T, _Float16>::value;      // (fp16's squares stay in range)
+    const float inv_d = 1.0f / (float)D, root_eps = sqrtf(a.eps), least = a.eps > 0.0f ? 0x1p-126f : 0.0f;
     // (the loop is uniform over the work-group, as its barriers need it: a group of threads without a row left works on zeros and stores nothing)
     for (long long r0 = (long long)blockIdx.x * RPG; r0 < a.rows; r0 += (long long)gridDim.x * RPG) {
         const long long r = r0 + t / NT;
@@ -172,29 +182,46 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_fwd_kernel(NormArgs 
         const long long rr = live ? r : a.rows - 1;
         float x[NV][8];
         row_load<T, NT, NV, WHOLE>(static_cast<const T*>(a.x) + rr * a.ldx, D, live ? D : 0, l, x);
-        float s = 0.0f;
+        // The row is evaluated times 2^-e, the power of two that brings the larger of max |x| and sqrt(eps) into [1, 2): its squares stay in fp32's range for
+        // all finite rows (unscaled they leave it from about 1e17 on, and below 1e-19 where eps does not cover them).  The scaling is exact, so ordinary rows
+        // have the bits they have without it.  (The maximum costs bf16 2 .. 6 % of the time, fp32 nothing; a rare second pass over such rows instead cost more
+        // in registers: 65536 x 512 bf16 23.0 us without, 24.5 with the maximum, 27 with a second pass.)
+        float s = 0.0f, top = 0.0f;
+        int e = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += x[i][j];
+            for (int j = 0; j < 8; ++j) {
+                s = SCALED ? fmaf(x[i][j], 0x1p-15f, s) : s + x[i][j];      // (2^14 values: the sum stays in range as well)
+                if constexpr (SCALED) top = fmaxf(top, fabsf(x[i][j]));
+            }
+        const float2 first = row_sum2<NT, SCALED>(s, top, red, t);
+        float mu = over(first.x, (float)D, inv_d), q = 0.0f, eps = a.eps;
+        if constexpr (SCALED) {
+            e = min((int)(__builtin_bit_cast(unsigned, fmaxf(first.y, root_eps)) >> 23) - 127, 126);
+            e = max(e, -126);
+            mu = ldexpf(mu, 15 - e);
+            eps = ldexpf(eps, -2 * e);
+        }
+        const float unit = SCALED ? __builtin_bit_cast(float, (unsigned)(127 - e) << 23) : 1.0f;
         // the mean's own rounding is taken out again: d = the mean of x - mu (a row without spread gives h = 0, not a last bit times 1 / sqrt(eps))
-        float mu = row_sum2<NT>(s, 0.0f, red, t).x / (float)D, q = 0.0f;
         s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[i][j] -= col_of<NT>(l, i) + (WHOLE ? 0 : j) < D ? mu : 0.0f;      // (columns beyond the row are 0 and stay 0)
+                x[i][j] = fmaf(x[i][j], unit, col_of<NT>(l, i) + (WHOLE ? 0 : j) < D ? -mu : 0.0f);      // (columns beyond the row are 0 and stay 0)
                 s += x[i][j];
                 q = fmaf(x[i][j], x[i][j], q);
             }
         const float2 c = row_sum2<NT>(s, q, red, t);
-        const float d = c.x * inv_d, rstd = 1.0f / sqrtf(fmaxf(fmaf(c.y, inv_d, -d * d), 0.0f) + a.eps);
-        mu += d;
+        const float d = over(c.x, (float)D, inv_d);       // (to the last bit: equal values cancel also where eps is nothing next to them)
+        const float scale = 1.0f / sqrtf(fmaxf(fmaxf(fmaf(c.y, inv_d, -d * d), 0.0f) + eps, least)), rstd = SCALED ? ldexpf(scale, -e) : scale;
+        mu = SCALED ? ldexpf(mu + d, e) : mu + d;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[i][j] = (x[i][j] - (col_of<NT>(l, i) + (WHOLE ? 0 : j) < D ? d : 0.0f)) * rstd;
+            for (int j = 0; j < 8; ++j) x[i][j] = (x[i][j] - (col_of<NT>(l, i) + (WHOLE ? 0 : j) < D ? d : 0.0f)) * scale;
         if (a.mean && live && l == 0) a.mean[r] = mu;
         if (a.rstd && live && l == 0) a.rstd[r] = rstd;
         if (a.codes) row_encode<NT, NV, WHOLE>(x, live ? D : 0, l, a.codes + r * D, a.exps + r * ((D + 31) >> 5));
@@ -231,11 +258,12 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void norm_bwd_kernel(NormArgs 
             row_decode<NT, NV, WHOLE>(a.codes + rr * D, a.exps + rr * ((D + 31) >> 5), D, n, l, h);
         } else {
             row_load<T, NT, NV, WHOLE>(static_cast<const T*>(a.x) + rr * a.ldx, D, n, l, h);
-            const float mu = a.mean[rr];
+            // (x - mu) rstd as (x / 2 - mu / 2) 2 rstd: the same bits, and the difference of two large values stays in range
+            const float half = 0.5f * a.mean[rr], twice = 2.0f * rstd;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] = (h[i][j] - mu) * rstd;        // (columns beyond the row: g = 0 there, so h does not matter)
+                for (int j = 0; j < 8; ++j) h[i][j] = fmaf(h[i][j], 0.5f, -half) * twice;        // (columns beyond the row: g = 0 there, so h does not matter)
         }
         float s = 0.0f, q = 0.0f;
 #pragma unroll

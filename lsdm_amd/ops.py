@@ -63,7 +63,8 @@ def linear(x, weight, bias=None, activation="none", residual=None, *, checkpoint
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, checkpoint8=False):
-    """Layer norm over the last axis: x (..., D), weight / bias (D) or None -> (..., D); D <= 16384.
+    """Layer norm over the last axis: x (..., D), weight / bias (D) or None -> (..., D); D <= 16384.  Rows of any finite values (their squares need not fit
+    the type); a row that holds an infinity or a NaN is NaN.
 
     ``checkpoint8`` (bfloat16 / float16): keep the normalised rows in 8 bits for the backward pass (the module docstring)."""
     return _lib.load_torch_ops().layer_norm(x, weight, bias, eps, bool(checkpoint8))
