@@ -95,8 +95,12 @@ __device__ __forceinline__ void store_param(void* p, int is_f32, long long i, fl
 }
 
 // ---- activations: y = a(z) and, where asked for, d = a'(z) ----
-// fp32 results use the libm functions; 16-bit results the hardware exp2 / reciprocal forms of common.hpp (absolute error <= 3e-7, four orders
-// below a bf16 step of a value near one).  NaN stays NaN in y for every activation; relu'(NaN) = 0 (the comparison z > 0).
+// fp32 results use the libm functions; 16-bit results the hardware's exp2 and reciprocal (1 ulp each), and for gelu Abramowitz & Stegun 7.1.26 (|error| of
+// Phi <= 1.5e-7, as in common.hpp); tanh is tanhf in every type.  Absolute error of the factors Phi and s <= 3e-7, of y = z Phi and z s |z| times that: in the
+// far tail of 16-bit gelu the polynomial's own error shows (1 % of y at z = -8, where y = -5e-15).  No form subtracts from one what may be next to one: 1 - s
+// is e s with e = exp(-c z) (its NaN at e = infinity, s = 0 gives way to 1), Phi of a negative z comes from erfc, 1 - tanh^2 from exp(-2 |z|); so fp32 values and
+// derivatives keep their relative accuracy in saturation (a few ulp, plus z^2 ulp for gelu).  NaN stays NaN in y for every activation; relu'(NaN) = 0 (the
+// comparison z > 0).
 template <class T, int ACT>
 __device__ __forceinline__ void act_one(float z, bool want, float& y, float& d) {
     constexpr bool fast = sizeof(T) == 2;
@@ -114,20 +118,20 @@ __device__ __forceinline__ void act_one(float z, bool want, float& y, float& d) 
         y = z * phi;
         d = fmaf(z * 0.39894228040143267794f, ex, phi);
     } else if constexpr (ACT == OP_GELU) {
-        const float phi = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+        const float phi = 0.5f * erfcf(z * -0.70710678118654752440f);
         y = z * phi;
         if (want) d = phi + z * 0.39894228040143267794f * expf(-0.5f * z * z);
-    } else if constexpr (ACT == OP_QUICK_GELU || ACT == OP_SILU) {
-        constexpr float c = ACT == OP_SILU ? 1.0f : 1.702f;
-        const float s = fast ? sigmoid_fast(c * z) : sigmoidf(c * z);
-        y = z * s;
-        d = s * fmaf(c * z, 1.0f - s, 1.0f);
-    } else if constexpr (ACT == OP_SIGMOID) {
-        y = fast ? sigmoid_fast(z) : sigmoidf(z);
-        d = y * (1.0f - y);
+    } else if constexpr (ACT == OP_QUICK_GELU || ACT == OP_SILU || ACT == OP_SIGMOID) {
+        constexpr float c = ACT == OP_QUICK_GELU ? 1.702f : 1.0f;
+        const float e = fast ? __expf(-(c * z)) : expf(-(c * z)), s = fast ? __builtin_amdgcn_rcpf(1.0f + e) : 1.0f / (1.0f + e), rest = fminf(e * s, 1.0f);
+        y = ACT == OP_SIGMOID ? s : z * s;
+        d = ACT == OP_SIGMOID ? s * rest : s * fmaf(c * z, rest, 1.0f);
     } else {
         y = tanhf(z);
-        d = fmaf(-y, y, 1.0f);
+        if (want) {
+            const float e = fast ? __expf(-2.0f * fabsf(z)) : expf(-2.0f * fabsf(z)), r = fast ? __builtin_amdgcn_rcpf(1.0f + e) : 1.0f / (1.0f + e);
+            d = 4.0f * e * r * r;
+        }
     }
 }
 template <class T, int ACT>

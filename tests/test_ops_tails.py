@@ -1,4 +1,7 @@
-"""The public operators where values are far from one: rows whose squares leave the range of fp32."""
+"""The public operators where values are far from one: saturated activations and their derivatives, rows whose squares leave the range of fp32.
+Every bound is added up from the roundings of the evaluation, relative to the value itself: u = 2^-24 for an fp32 operation."""
+import math
+
 import pytest
 import torch
 
@@ -6,13 +9,67 @@ import test_ops as base
 from lsdm_amd import ops
 
 gpu = pytest.mark.gpu
-DEV, DT = base.DEV, base.DT
+DEV, U, DT = base.DEV, base.U, base.DT
+half_step, within = base.half_step, base.within
 
 
 @pytest.fixture(autouse=True)
 def _grad_mode():
     with torch.enable_grad():
         yield
+
+
+def through(act, z, dt, checkpoint8=False):
+    """y = a(z) and a'(z) as the operator has them: z comes in as an fp32 bias under an input of zeros, one row, and a'(z) out as the bias' gradient, which is
+    summed in fp32 and not rounded to the operands' type."""
+    t = DT[dt]
+    x, w = torch.zeros(1, 1, device=DEV, dtype=t), torch.ones(z.numel(), 1, device=DEV, dtype=t)
+    b = z.to(DEV, torch.float32).clone().requires_grad_(True)
+    y = ops.linear(x, w, b, act, checkpoint8=checkpoint8)
+    (d,) = torch.autograd.grad(y, [b], torch.ones_like(y))
+    return y.detach().view(-1), d
+
+
+def phi64(z):
+    """The normal distribution function through erfc (torch's ndtr is 1 + erf, which is 0 from z = -8.3 on)."""
+    return 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+
+
+def act64(act, z):
+    if act == "gelu":
+        return z * phi64(z), phi64(z) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return base.act64(act, z)
+
+
+def grid(lo, hi, n=4001):
+    return torch.linspace(lo, hi, n).float()
+
+
+# fp32: y and a' relative to the value.  exp of an exact argument and a division are off by a few u; where the argument itself is a rounded product p
+# (gelu: z / sqrt(2), z^2 / 2), its rounding costs |p|' s change of the logarithm, 2 u z^2 for both of gelu's factors.  The two terms of a'(z) may cancel, so
+# its bound goes by their magnitudes.
+@gpu
+@pytest.mark.parametrize("act,lo,hi", [("gelu", -9.0, -2.0), ("gelu", 2.0, 9.0), ("sigmoid", -60.0, -3.0), ("sigmoid", 3.0, 60.0), ("tanh", -30.0, -1.0), ("tanh", 1.0, 30.0),
+                                       ("silu", -60.0, -3.0), ("silu", 3.0, 60.0), ("quick_gelu", -40.0, -2.0), ("quick_gelu", 2.0, 40.0)])
+def test_tails_in_fp32(act, lo, hi):
+    z = grid(lo, hi)
+    y, d = through(act, z, "f32")
+    z = z.to(DEV).double()
+    want_y, want_d = act64(act, z)
+    if act == "gelu":
+        pdf = z.abs() * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+        phi = phi64(z)
+        ry, sd = 2 * z * z + 16, (2 * z * z + 16) * (phi + pdf)
+    elif act in ("silu", "quick_gelu"):
+        c = 1.702 if act == "quick_gelu" else 1.0
+        s = torch.special.expit(c * z)
+        ry = 16 + 2 * c * z.abs()                          # (1.702 z is a rounded product)
+        sd = ry * s * (1 + c * z.abs() * torch.special.expit(-c * z))
+    else:
+        ry = torch.full_like(z, 16.0)
+        sd = ry * want_d
+    within(y, want_y, ry * U * want_y.abs(), "y")
+    within(d, want_d, sd * U, "a'")
 
 
 # ------------------------------------------------------------------------------------------------ layer norm: squares beyond fp32's range
