@@ -247,7 +247,7 @@ enum {
 
 /* y = a(x w^T + bias) + residual.  x (M,K) with row stride ldx, w (N,K) with row stride ldw, bias (N) or NULL, residual (M,N) with row stride
  * ldr or NULL (it may be y itself), y (M,N) dense.  deriv: NULL, or (M,N) that receives a'(z) for lsdm_linear_backward (untouched without an
- * activation): fp32 in fp32 calls, a 16-bit form (sign, 3 exponent bits, 12 mantissa bits) in bf16 / fp16 calls, or LSDM_OP_DERIV8's bytes.
+ * activation): fp32 in fp32 calls, a 16-bit form (sign, and 31744 |a'|^(1/4) as a whole number) in bf16 / fp16 calls, or LSDM_OP_DERIV8's bytes.
  * 1 <= M, K <= 2^30, 1 <= N <= 2^25. */
 LSDM_API int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
                 int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, void* deriv, void* ws, int64_t ws_bytes, void* stream);

@@ -10,7 +10,8 @@ the tensors' device (argument checks, allocation and autograd nodes: csrc/torch_
 
 Types: float32, bfloat16, float16, the same for all tensors of a call (``bias`` and the norm's ``weight`` / ``bias`` may also be float32).  Products
 accumulate and everything else is evaluated in 32 bits; results are rounded once.  In 16 bits the backward pass of ``linear`` rounds dz = dy a'(z) to the
-tensors' type, as the matrix cores take their operands in it (a'(z) itself is kept with 13 significant bits).
+tensors' type, as the matrix cores take their operands in it (a'(z) itself is kept in 16 bits that round it by 2^-14 of its value near 1,
+2^-13 at 1/16 and 2^-8 at 1e-7).
 Shapes: any leading axes, any sizes including 0 rows (at most 2^30 rows and columns, 2^25 rows of ``weight``, 2^35 values of a checkpoint); the last axis should be contiguous (other layouts are copied first).
 Gradients are differentiable once; forward-mode derivatives there are none (a dual tensor raises ``LsdmError``).  Results do not depend on timing (no atomics): the same call gives the same bits.
 

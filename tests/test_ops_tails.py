@@ -72,6 +72,49 @@ def test_tails_in_fp32(act, lo, hi):
     within(d, want_d, sd * U, "a'")
 
 
+# 16 bits: a'(z) is kept in a form that is never coarser than half a step of bf16 (2^-8 of the value) down to 2^-23, and 2^-6 down to 2^-31.7; the functions
+# themselves are good to 1e-4 of their terms over these ranges (gelu: 7.1.26's polynomial far out; the others: exp2 of a rounded product).
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("act,lo,hi", [("gelu", -5.6, -0.9), ("sigmoid", -22.0, 0.0), ("sigmoid", 0.0, 22.0), ("tanh", -11.0, 0.0), ("tanh", 0.0, 11.0), ("silu", -25.0, -1.5),
+                                       ("quick_gelu", -15.0, -1.0)])
+def test_small_derivatives_in_16_bits(act, lo, hi, dt):
+    z = grid(lo, hi)
+    _, d = through(act, z, dt)
+    z = z.to(DEV).double()
+    _, want = act64(act, z)
+    terms = want.abs()
+    if act == "gelu":
+        terms = phi64(z) + z.abs() * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    elif act in ("silu", "quick_gelu"):
+        c = 1.702 if act == "quick_gelu" else 1.0
+        terms = torch.special.expit(c * z) * (1 + c * z.abs())
+    rel = torch.where(want.abs() >= 2.0 ** -23, 2.0 ** -8, 2.0 ** -6)
+    within(d, want, rel * want.abs() + 1e-4 * terms + 2.0 ** -40, "a'")
+    assert bool((d != 0).all() | (want.abs() < 2.0 ** -40).any())
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_kept_derivatives_near_one(dt):
+    """... and a'(z) itself keeps 2^-13 of the value from 1/32 up, 0 and 1 exactly, and NaN."""
+    for act in ("gelu", "quick_gelu", "silu", "sigmoid", "tanh"):
+        z = grid(-1.5, 4.0)
+        _, d = through(act, z, dt)
+        _, want = act64(act, z.to(DEV).double())
+        big = want.abs() >= 1.0 / 32
+        within(d[big], want[big], 2.0 ** -13 * want[big].abs() + 1.2e-6 * (1 + z.to(DEV).double()[big].abs()), act)
+    _, d = through("relu", torch.tensor([-3.0, -0.0, 0.0, 1e-30, 5.0, float("inf"), -float("inf")]), dt)
+    assert d.tolist() == [0, 0, 0, 1, 1, 1, 0]
+    for act in ("gelu", "quick_gelu", "silu", "sigmoid", "tanh"):
+        _, d = through(act, torch.tensor([float("nan"), 1.0]), dt)
+        assert bool(d[0].isnan()) and bool(d[1].isfinite())
+    for act, ends in (("sigmoid", [0, 0]), ("tanh", [0, 0])):
+        for inf in (float("inf"), 1e30):
+            y, d = through(act, torch.tensor([-inf, inf]), dt)
+            assert d.tolist() == ends and y[1] == 1
+
+
 # ------------------------------------------------------------------------------------------------ layer norm: squares beyond fp32's range
 WIDTHS = [3, 8, 40, 64, 100, 256, 300, 512, 771, 1024, 1500, 2048, 2051, 4096, 5001, 8192, 16384]
 
