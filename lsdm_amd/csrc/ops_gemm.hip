@@ -4,8 +4,8 @@
 //   dx        dz W                          A = dz, B(n, k) = W[k][n]: contiguous in A only                                               (KM)
 //   dW        dz^T x                        A(m, k) = dz[k][m], B(n, k) = x[k][n]: contiguous in neither                                  (MM)
 //
-// One tile core for all three.  A work-group owns a BM x BN tile of C and walks k in steps of SB = 64 or 128 bytes: both operand tiles come into LDS by
-// LDS-DMA (16 bytes per lane, no registers), the next steps' in flight while this one is multiplied.
+// One tile core for all three.  A work-group owns a BM x BN tile of C and walks k in steps of 128 bytes through two LDS buffers: both operand tiles come into
+// LDS by LDS-DMA (16 bytes per lane, no registers), the next step's in flight while this one is multiplied.
 //   16-bit: v_mfma_f32_16x16x32; a tile whose contraction axis is contiguous is read with ds_read_b128, the other kind with the transposing
 //           ds_read_b64_tr_b16, so that no operand is ever transposed in memory.
 //   fp32:   v_mfma_f32_32x32x2 (exact products, an fmaf chain).
@@ -17,7 +17,7 @@
 // Measured (MI355X, back to back): 8192 x 4096 x 8256 bf16 KK 428 us = 1.30 PFLOP/s (a 16 KiB row stride, K = 8192, costs 15 %: the rows of a tile fall on
 // the same channels), 16384 x 2048 x 8192 KM 448 us = 1.23, 8192 x 2048 x 8192 MM 203 us = 1.36; fp32 4096^3 KM 1.05 ms = 0.131.  Bound by the issue of
 // the LDS copies next to the matrix instructions (SQ_VALU_MFMA_BUSY 57 % of the cycles); with all rows on one cache line the same loop reaches 1.38.
-// Two 128-byte steps in flight; 64-byte steps three to five deep, or two groups of waves half a period apart, measured 0 .. 15 % slower.
+// 64-byte steps in three to five buffers, or two groups of waves half a period apart, measured 0 .. 15 % slower.
 #include <algorithm>
 
 #include "ops.hpp"
@@ -51,18 +51,16 @@ template <> struct Mma<float> {
 };
 
 // ---- LDS tiles ----------------------------------------------------------------------------------------------------------------
-// A step is SB bytes of the contraction axis.
+// A step is SB = 128 bytes of the contraction axis.
 // KMAJOR: R rows of SB bytes, the 16-byte chunk c of row r at position c ^ swz(r).
 // else:   SB / sizeof(T) rows (one per k) of R elements; a block of 16 columns (32 bytes, 16-bit types) or 32 columns (128 bytes, fp32) b of
 //         row k at position b ^ swz(k).
 // ds_read_b128 takes its 64 lanes in four passes over the 64 banks: lanes 0-3, 12-15, 20-27; 4-11, 16-19, 28-31; and the same 32 lanes further.
 // The sixteen rows (fp32: chunks) of a pass fall into sixteen different 16-byte columns of the banks with these two forms (SQ_LDS_BANK_CONFLICT
 // from 50 % of the LDS cycles with r & 7 and (r >> 2) & 3 to 0).
-template <class T, int SB>
-__device__ __forceinline__ int swz_k(int r) {
-    if constexpr (SB == 64) return ((r >> 3) & 1) * 2;
-    else return ((r >> 1) & 1) * 2 | ((r >> 3) & 1) * 4 | (sizeof(T) == 4 ? (r >> 4) & 1 : 0);
-}
+constexpr int SB = 128;
+template <class T>
+__device__ __forceinline__ int swz_k(int r) { return ((r >> 1) & 1) * 2 | ((r >> 3) & 1) * 4 | (sizeof(T) == 4 ? (r >> 4) & 1 : 0); }
 template <class T, int R>
 __device__ __forceinline__ int swz_m(int k) {
     if constexpr (sizeof(T) == 4) return (k >> 2) & 1;
@@ -70,7 +68,7 @@ __device__ __forceinline__ int swz_m(int k) {
     else return ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
 }
 
-template <class T, int R, bool KMAJOR, int NW, int SB>
+template <class T, int R, bool KMAJOR, int NW>
 struct Loader {
     static constexpr int NI = R * SB / 1024 / NW;        // wave instructions (1 KB each) per wave and step
     static constexpr int EC = 16 / (int)sizeof(T), CPR = SB / 16;
@@ -86,7 +84,7 @@ struct Loader {
         for (int i = 0; i < NI; ++i) {
             const int q = wave * NI + i;
             if constexpr (KMAJOR) {
-                const int r = q * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ swz_k<T, SB>(r);
+                const int r = q * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ swz_k<T>(r);
                 const int gr = min(row0 + r, rows - 1);
                 kpos[i] = c * EC;
                 src[i] = reinterpret_cast<const char*>(p + (long long)gr * ld + k0 + c * EC);
@@ -117,7 +115,7 @@ struct Loader {
 };
 
 // fragments of one wave: NF blocks of F rows starting at row0 of the tile
-template <class T, int R, bool KMAJOR, int NF, int SB>
+template <class T, int R, bool KMAJOR, int NF>
 struct Reader {
     typedef Mma<T> MM_;
     typedef typename MM_::frag frag;
@@ -129,7 +127,7 @@ struct Reader {
         if constexpr (sizeof(T) == 2 && KMAJOR) {
             const int r = row0 + (lane & 15);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) off[s] = r * SB + (((s * 4 + (lane >> 4)) ^ swz_k<T, SB>(r)) << 4);
+            for (int s = 0; s < KS; ++s) off[s] = r * SB + (((s * 4 + (lane >> 4)) ^ swz_k<T>(r)) << 4);
         } else if constexpr (sizeof(T) == 2) {
             const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
@@ -137,7 +135,7 @@ struct Reader {
         } else if constexpr (KMAJOR) {
             const int r = row0 + (lane & 31);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) off[s] = r * SB + (((2 * s + (lane >> 5)) ^ swz_k<T, SB>(r)) << 4);
+            for (int s = 0; s < KS; ++s) off[s] = r * SB + (((2 * s + (lane >> 5)) ^ swz_k<T>(r)) << 4);
         } else {
             frow = row0;
         }
@@ -244,14 +242,14 @@ __global__ __launch_bounds__(256) void colsum_join_kernel(GemmArgs g) {
 }
 
 // ---- the tile kernel ------------------------------------------------------------------------------------------------------------
-template <class T, int BM, int BN, int WGM, int WGN, int STAGES, int SB, bool AKM, bool BKM, int WPE>
+template <class T, int BM, int BN, int WGM, int WGN, bool AKM, bool BKM, int WPE>
 __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
     typedef Mma<T> MM_;
     constexpr int NW = WGM * WGN, TM = BM / WGM, TN = BN / WGN, F = MM_::F, FM = TM / F, FN = TN / F;
-    constexpr int BK = SB / (int)sizeof(T), KS = Reader<T, BM, AKM, FM, SB>::KS;
+    constexpr int BK = SB / (int)sizeof(T), KS = Reader<T, BM, AKM, FM>::KS;
     constexpr int TA = BM * SB, TB = BN * SB, ST = TA + TB;
     constexpr int RW = TM < 64 ? TM : 64, PITCH = TN * 4 + 16, EPI = RW * PITCH;        // epilogue: RW rows of a wave's tile at a time, in fp32
-    constexpr int BYTES = ST * STAGES > EPI * NW ? ST * STAGES : EPI * NW;
+    constexpr int BYTES = 2 * ST > EPI * NW ? 2 * ST : EPI * NW;
     __shared__ __attribute__((aligned(1024))) char lds[BYTES];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave / WGN, wn = wave - wm * WGN;
@@ -269,12 +267,12 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
     const int k_lo = ks * g.kchunk, k_hi = min(g.K, k_lo + g.kchunk);
     const int nk = k_hi > k_lo ? (k_hi - k_lo + BK - 1) / BK : 0;
 
-    Loader<T, BM, AKM, NW, SB> la;
-    Loader<T, BN, BKM, NW, SB> lb;
+    Loader<T, BM, AKM, NW> la;
+    Loader<T, BN, BKM, NW> lb;
     la.init(g.A, g.lda, m0, g.M, k_lo, wave, lane);
     lb.init(g.B, g.ldb, n0, g.N, k_lo, wave, lane);
-    Reader<T, BM, AKM, FM, SB> ra;
-    Reader<T, BN, BKM, FN, SB> rb;
+    Reader<T, BM, AKM, FM> ra;
+    Reader<T, BN, BKM, FN> rb;
     ra.init(wm * TM, lane);
     rb.init(wn * TN, lane);
     const unsigned base = lds_addr(lds);
@@ -287,32 +285,16 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
 #pragma unroll
             for (int r = 0; r < (int)(sizeof(typename MM_::acc) / 4); ++r) acc[i][j][r] = 0.0f;
 
-    int issued = 0;
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s)
-        if (issued < nk) {
-            la.issue(base + s * ST, wave, k_hi - k_lo - issued * BK);
-            lb.issue(base + s * ST + TA, wave, k_hi - k_lo - issued * BK);
-            ++issued;
-        }
-    constexpr int PER = Loader<T, BM, AKM, NW, SB>::NI + Loader<T, BN, BKM, NW, SB>::NI;      // LDS-DMA instructions per wave and step
-    auto issue_next = [&](int buf) {
-        la.issue(base + buf * ST, wave, k_hi - k_lo - issued * BK);
-        lb.issue(base + buf * ST + TA, wave, k_hi - k_lo - issued * BK);
-        ++issued;
+    auto issue = [&](int buf, int it) {
+        la.issue(base + buf * ST, wave, k_hi - k_lo - it * BK);
+        lb.issue(base + buf * ST + TA, wave, k_hi - k_lo - it * BK);
     };
-    // waits until at most `younger` steps' pieces of this wave are in flight
-    auto wait_landed = [&](int younger) {
-        if (younger <= 0) lds_dma_wait();
-        else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
-    };
+    if (nk > 0) issue(0, 0);
     int buf = 0;
     for (int it = 0; it < nk; ++it) {
-        // this step's pieces have landed (the younger steps' may still be on their way), for every wave behind the barrier
-        wait_landed(min(issued - it - 1, STAGES - 2));
+        lds_dma_wait();                          // this step's pieces have landed, for every wave behind the barrier
         wg_sync();
-        if (issued < nk) issue_next(buf == 0 ? STAGES - 1 : buf - 1);       // the buffer of step it - 1, which every wave has read
+        if (it + 1 < nk) issue(buf ^ 1, it + 1); // into the buffer of step it - 1, which every wave has read
         const char* ta = lds + buf * ST;
         const char* tb = ta + TA;
 #pragma unroll
@@ -343,7 +325,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, WPE) void gemm_kernel(GemmArgs g) {
             }
             __builtin_amdgcn_sched_group_barrier(0x8, MF - PERR * (READS - AHEAD), 0);
         }
-        buf = buf + 1 == STAGES ? 0 : buf + 1;
+        buf ^= 1;
     }
 
     // epilogue: the wave's tile through its own piece of LDS, RW rows at a time
@@ -580,12 +562,12 @@ __global__ __launch_bounds__(256) void prep_kernel(PrepArgs args) {
 // ---- host side ------------------------------------------------------------------------------------------------------------------
 namespace {
 
-template <class T, int BM, int BN, int WGM, int WGN, int STAGES, int SB, int WPE>
+template <class T, int BM, int BN, int WGM, int WGN, int WPE>
 void launch_layout(const GemmArgs& g, int layout, unsigned grid, hipStream_t st) {
     const dim3 b(64 * WGM * WGN);
-    if (layout == KK) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, SB, true, true, WPE>), dim3(grid), b, 0, st, g);
-    else if (layout == KM) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, SB, true, false, WPE>), dim3(grid), b, 0, st, g);
-    else hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, STAGES, SB, false, false, WPE>), dim3(grid), b, 0, st, g);
+    if (layout == KK) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, true, true, WPE>), dim3(grid), b, 0, st, g);
+    else if (layout == KM) hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, true, false, WPE>), dim3(grid), b, 0, st, g);
+    else hipLaunchKernelGGL((gemm_kernel<T, BM, BN, WGM, WGN, false, false, WPE>), dim3(grid), b, 0, st, g);
 }
 
 }  // namespace
@@ -596,11 +578,11 @@ void launch_gemm_t(const GemmPlan& p, GemmArgs g, int layout, hipStream_t st) {
     g.blocks = p.tiles_m * p.tiles_n * p.splits;
     const unsigned grid = (unsigned)(g.blocks + (g.cs_out ? (g.cs_n + 63) / 64 : 0));
     if constexpr (sizeof(T) == 2) {
-        if (p.tile == 256) launch_layout<T, 256, 256, 2, 4, 2, 128, 2>(g, layout, grid, st);
-        else if (p.tile < p.tile_n) launch_layout<T, 64, 128, 2, 2, 2, 128, 2>(g, layout, grid, st);
+        if (p.tile == 256) launch_layout<T, 256, 256, 2, 4, 2>(g, layout, grid, st);
+        else if (p.tile < p.tile_n) launch_layout<T, 64, 128, 2, 2, 2>(g, layout, grid, st);
     }
-    if (p.tile == 128) launch_layout<T, 128, 128, 2, 2, 2, 128, 2>(g, layout, grid, st);
-    else if (p.tile_n == 64) launch_layout<T, 64, 64, 2, 2, 2, 128, 2>(g, layout, grid, st);
+    if (p.tile == 128) launch_layout<T, 128, 128, 2, 2, 2>(g, layout, grid, st);
+    else if (p.tile_n == 64) launch_layout<T, 64, 64, 2, 2, 2>(g, layout, grid, st);
     if (p.splits > 1) {
         const int ppr = (g.N + 7) / 8;
         const long long pieces = (long long)g.M * ppr;
