@@ -260,6 +260,9 @@ LSDM_API int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, i
                 int64_t ws_bytes, void* stream);
 /* bytes of scratch memory of either call (flags: the enum above), or a negative lsdm_status */
 LSDM_API int64_t lsdm_linear_workspace(int dtype, int flags, int64_t M, int64_t N, int64_t K);
+/* Test hook: the tile that evaluates an (M,N) product with a contraction of K (y: M, N, K; dx: M, K, N; dw: N, K, M), as rows << 32 | columns << 16 | parts
+ * of the contraction; 0 if no launch can hold the tiles.  (Products of up to 64 rows run on another kernel in lsdm_linear.) */
+LSDM_API int64_t lsdm_linear_plan(int dtype, int64_t M, int64_t N, int64_t K);
 
 /* y = (x - mean) / sqrt(var + eps) * w + b over the last axis, var = mean (x - mean)^2.  x (rows,D) with row stride ldx, y (rows,D) dense, w and b
  * (D) or NULL (1 and 0), 1 <= D <= 16384.  For the backward pass: mean, rstd (rows) fp32 or NULL; codes (rows,D) int8 with exps

@@ -56,6 +56,7 @@ _SIGNATURES = {
     "lsdm_linear": (_i, [_i] * 4 + [_i64] * 3 + [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
     "lsdm_linear_backward": (_i, [_i] * 3 + [_i64] * 3 + [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
     "lsdm_linear_workspace": (_i64, [_i] * 2 + [_i64] * 3),
+    "lsdm_linear_plan": (_i64, [_i] + [_i64] * 3),
     "lsdm_layer_norm": (_i, [_i] * 3 + [_i64] * 2 + [_vp, _i64, _vp, _vp, _f] + [_vp] * 6),
     "lsdm_layer_norm_backward": (_i, [_i] * 3 + [_i64] * 2 + [_vp, _i64, _vp, _i64] + [_vp] * 9 + [_i64, _vp]),
     "lsdm_layer_norm_workspace": (_i64, [_i64] * 2),

@@ -197,6 +197,12 @@ int64_t lsdm_linear_workspace(int dtype, int flags, int64_t M, int64_t N, int64_
                            !(flags & LSDM_OP_DY_UNALIGNED), x_ok, w_ok, nullptr).bytes;
 }
 
+int64_t lsdm_linear_plan(int dtype, int64_t M, int64_t N, int64_t K) {
+    if (check_linear(dtype, M, N, K) != LSDM_OK) return LSDM_ERR_ARG;
+    const GemmPlan p = plan(M, N, K, dtype);
+    return (int64_t)p.tile << 32 | (int64_t)p.tile_n << 16 | (p.tile ? p.splits : 0);
+}
+
 int lsdm_linear(int device, int dtype, int activation, int flags, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w, int64_t ldw,
                 const void* bias, const void* residual, int64_t ldr, void* y, void* deriv, void* ws, int64_t ws_bytes, void* stream) {
     if (const int rc = check_linear(dtype, M, N, K)) return rc;
