@@ -7,6 +7,7 @@ import ctypes as C
 import importlib.machinery
 import importlib.util
 import os
+import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liblsdm_hip.so")
@@ -87,20 +88,27 @@ def load():
 
 
 _torch_ops = None
+_torch_ops_lock = threading.Lock()       # (a second load beside the first would be a second module)
+
+
+def _load_torch_ops():
+    load()
+    path = os.path.join(_HERE, "_torch_ops.so")
+    if not os.path.exists(path):
+        raise LsdmError("_torch_ops.so not found at %s -- build it with `make -C lsdm_amd/csrc` (the operators have no other front end)" % path)
+    loader = importlib.machinery.ExtensionFileLoader("_torch_ops", path)
+    module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_torch_ops", loader, origin=path))
+    loader.exec_module(module)
+    return module
 
 
 def load_torch_ops():
     """Loads _torch_ops.so, the tensor front end of the public operators (csrc/torch_ops.cpp; built with the library)."""
     global _torch_ops
     if _torch_ops is None:
-        load()
-        path = os.path.join(_HERE, "_torch_ops.so")
-        if not os.path.exists(path):
-            raise LsdmError("_torch_ops.so not found at %s -- build it with `make -C lsdm_amd/csrc` (the operators have no other front end)" % path)
-        loader = importlib.machinery.ExtensionFileLoader("_torch_ops", path)
-        module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_torch_ops", loader, origin=path))
-        loader.exec_module(module)
-        _torch_ops = module
+        with _torch_ops_lock:
+            if _torch_ops is None:
+                _torch_ops = _load_torch_ops()
     return _torch_ops
 
 

@@ -1,4 +1,7 @@
 """How the public operators are called: under a tracer, with forward-mode derivatives, while a graph is captured, from several threads."""
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -115,6 +118,26 @@ def test_capture_with_a_live_eager_graph_behind_the_inputs_is_refused():
         assert all(torch.equal(a, b) for a, b in zip(taken, want))
     torch.autograd.grad(alive[0], [w, b], torch.ones_like(alive[0]))      # the eager graphs are as they were
     torch.autograd.grad(alive[1], [n], torch.ones_like(alive[1]))
+
+
+def test_first_calls_of_several_threads_load_one_front_end():
+    """In a process of its own, with threads that change places at every step."""
+    code = """
+import sys, threading
+sys.setswitchinterval(1e-6)
+import torch
+from lsdm_amd import _lib
+at, found = threading.Barrier(8), []
+def run():
+    at.wait()
+    found.append(id(_lib.load_torch_ops()))
+threads = [threading.Thread(target=run) for _ in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert len(found) == 8 and len(set(found)) == 1, found
+"""
+    for _ in range(3):
+        subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=120)
 
 
 @gpu
