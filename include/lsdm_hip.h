@@ -278,7 +278,8 @@ LSDM_API int64_t lsdm_layer_norm_workspace(int64_t rows, int64_t D);
 
 /* 8-bit checkpoint of x (rows,D), row stride ldx: groups of 32 consecutive values of a row share the step 2^e, e = max(floor(log2 max|x|) - 6,
  * -126): codes (rows,D) int8 = x / 2^e rounded to nearest even, clamped to +-127; exps (rows,ceil(D/32)) uint8 = e + 127, or 255 for a group that
- * holds an infinity or a NaN.  lsdm_unpack8 writes the values codes 2^e (exact in every dtype; NaN where exps is 255) to out (rows,D) dense. */
+ * holds an infinity or a NaN.  lsdm_unpack8 writes the values codes 2^e (exact in x's dtype, LSDM_BF16 and LSDM_F32; NaN where exps is 255) to out
+ * (rows,D) dense. */
 LSDM_API int lsdm_pack8(int device, int dtype, int64_t rows, int64_t D, const void* x, int64_t ldx, void* codes, void* exps, void* stream);
 LSDM_API int lsdm_unpack8(int device, int dtype, int64_t rows, int64_t D, const void* codes, const void* exps, void* out, void* stream);
 

@@ -154,8 +154,9 @@ __device__ __forceinline__ void act8(int act, const float (&z)[8], bool want, fl
 
 // a'(z) is kept for the backward pass in 16 bits (bf16 and fp16 calls; fp32 calls keep fp32): the sign and C |a'|^(1/4) as a whole number, C = 31744; the
 // largest |a'|, gelu's 1.13, is code 32722.  A value d is rounded by 2 d / (C d^(1/4)): 2^-14 relative near 1, 2^-13 at 2^-4, and 2^-8, half a step of bf16, at
-// 2^-23; an eighth (bf16) and a half (fp16) of the type's own rounding where most derivatives lie, no zero before 2^-64.  (Sign, 3 exponent and 12 mantissa bits,
-// which ended at 2^-19, lost saturated derivatives.  Two square roots when written, three products when read: 16384 x 2048 -> 8192 with gelu, both passes, 1603 -> 1611 us.)
+// 2^-23; from 1/32 up a sixteenth (bf16) or a third (fp16) of half a step of the type itself, and no zero before 2^-64.  (Sign, 3 exponent and 12 mantissa
+// bits, which ended at 2^-19, lost saturated derivatives.  Two square roots when written, three products when read: 16384 x 2048 -> 8192 with gelu, both passes,
+// 1603 -> 1611 us.)
 // 0 and 1 (relu) are exact, as C (1 / C) is in fp32.  0x7fff stands for NaN.
 constexpr float kDeriv16 = 31744.0f;
 __device__ __forceinline__ unsigned deriv_code16(float d) {
@@ -183,7 +184,7 @@ enum DerivForm { DERIV_NONE = 0, DERIV_F32 = 1, DERIV_16 = 2, DERIV_8 = 3 };
 // ---- 8-bit checkpoint: groups of kGroup8 consecutive values of a row share a power-of-two step 2^e ----
 // m = max |x| of the group, e = max(floor(log2 m) - 6, -126), q = clamp(rint(x 2^-e), +-127); stored: q (int8), e + 127 (uint8), 255 for a
 // group that holds an infinity or a NaN (it decodes to NaN: a checkpoint never hides an overflow).  q 2^e has at most 7 significant bits, so it
-// is exact in fp32, bf16 and fp16.
+// is exact in fp32, in bf16 and in the type the values came from (in fp16 what lies outside its range is not, if they came from another).
 constexpr int kGroup8 = 32;
 constexpr unsigned kNanExp8 = 255u;
 __device__ __forceinline__ unsigned exp8_of_amax(float m) {        // m >= 0, NaN or inf for a non-finite group
@@ -191,11 +192,12 @@ __device__ __forceinline__ unsigned exp8_of_amax(float m) {        // m >= 0, Na
     return E == 255 ? kNanExp8 : (unsigned)(E - 6 > 1 ? E - 6 : 1);
 }
 __device__ __forceinline__ float exp8_step(unsigned b) { return b == kNanExp8 ? __builtin_nanf("") : __builtin_bit_cast(float, b << 23); }
-// 2^-e: e + 127 in [1, 248] -> the reciprocal's biased exponent 254 - b is in [6, 253]; b = 255 gives 0 (codes of such a group are 0)
+// 2^-e: e + 127 in [1, 248] -> the reciprocal's biased exponent 254 - b is in [6, 253]; b = 255 gives 0 (the codes of such a group: 0, or -127 for the
+// infinities and NaN themselves; nothing reads them as values)
 __device__ __forceinline__ float exp8_inv(unsigned b) { return b == kNanExp8 ? 0.0f : __builtin_bit_cast(float, (254u - b) << 23); }
 __device__ __forceinline__ int code8(float x, float inv) {
     const float v = rintf(x * inv);
-    return (int)fminf(fmaxf(v, -127.0f), 127.0f);                   // (non-finite groups: inv = 0, the NaN of inf * 0 is dropped by fmaxf)
+    return (int)fminf(fmaxf(v, -127.0f), 127.0f);                   // (non-finite groups: inv = 0, and the NaN of inf * 0 becomes -127)
 }
 
 // ---- kernels' argument blocks and launchers ----

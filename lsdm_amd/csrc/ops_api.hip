@@ -69,8 +69,10 @@ struct Carve {
 // 128-byte step of the contraction takes max(alone, shared * n) us with n of them there, prologue and epilogue fixed + each * n us.  The grid runs
 // in full rounds of 256 `resident` work-groups and a last, thinner one; a split contraction adds the join's launch and its traffic (the partial sums
 // are written once and read once).  The constants are fitted to timed launches of every tile and 1 .. 32 splits in the three operand layouts (16 bits:
-// 177 shapes log-uniform over 16 .. 16384; fp32: 35): the estimate's choice is within 1 % of the best one in the mean, within 20 % at worst.  Without
-// the 64 x 128 tile it would be 1.5 % (4928 x 2048 x 512: 22 -> 18 us, 704 x 1640 x 3952: 37 -> 25).
+// 177 shapes log-uniform over 16 .. 16384; fp32: 35) of products WITHOUT activation and derivative: among those the estimate's choice is within 1 % of the best
+// one in the mean, within 20 % at worst.  Without the 64 x 128 tile it would be 1.5 % (4928 x 2048 x 512: 22 -> 18 us, 704 x 1640 x 3952: 37 -> 25).  What an
+// epilogue costs is not in the estimate, though it is a third of a large product with gelu and its derivative: 8192 x 1024 -> 4096 runs 114 us where 62 are
+// expected, and another tile takes 98.
 struct TileCost { int tile, tile_n, resident; float alone, shared, fixed, each; };
 const TileCost kHalfTiles[] = {{256, 256, 1, 0.0f, 1.36f, 8.5f, 0.61f}, {128, 128, 2, 0.78f, 0.39f, 1.87f, 1.4f}, {64, 128, 3, 0.395f, 0.28f, 1.98f, 0.74f},
                                {64, 64, 5, 0.315f, 0.19f, 2.31f, 0.08f}};
@@ -258,8 +260,10 @@ int lsdm_linear_backward(int device, int dtype, int flags, int64_t M, int64_t N,
     OnDevice dev(device);
     if (!dev.ok) return LSDM_ERR_HIP;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // one launch prepares everything: dz = dy a'(z) in the operand's type (the matrix instruction's operand) with the column sums of its fp32 values,
-    // x from its 8-bit checkpoint, and rows that need padding
+    // one launch prepares everything: dz = dy a'(z) with the column sums of its fp32 values, x from its 8-bit checkpoint, and rows that need padding.
+    // dz is rounded to the operands' type: the matrix cores take both operands of a product in it, as an eager layer's backward pass does.  It puts a second
+    // rounding beside the result's (bf16, 16384 x 2048 -> 8192 with gelu: dx and dw 2.35e-3 from 64 bits, 1.66e-3 if dz were kept in 32); dz as two bf16 terms
+    // would take it out again and double both products, 900 us more in a pass of 1600.  Derivatives of 0 and 1 (relu, none) round nothing.
     PrepArgs prep;
     int jobs = 0;
     GemmArgs base;

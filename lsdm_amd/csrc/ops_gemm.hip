@@ -14,9 +14,10 @@
 // LDS-DMA writes lane l's 16 bytes at base + 16 l, so the bank swizzle is put into the GLOBAL address a lane reads (src_* below) and undone by
 // the reader.  A lane whose k lies beyond the end reads 16 zero bytes (g_zero16); rows beyond the end are clamped to the last one, and their
 // results are not stored.
-// Measured (MI355X, back to back): 8192 x 4096 x 8256 bf16 KK 428 us = 1.30 PFLOP/s (a 16 KiB row stride, K = 8192, costs 15 %: the rows of a tile fall on
-// the same channels), 16384 x 2048 x 8192 KM 448 us = 1.23, 8192 x 2048 x 8192 MM 203 us = 1.36; fp32 4096^3 KM 1.05 ms = 0.131.  Bound by the issue of
-// the LDS copies next to the matrix instructions (SQ_VALU_MFMA_BUSY 57 % of the cycles); with all rows on one cache line the same loop reaches 1.38.
+// Measured (MI355X, back to back; the boxes differ by 5 %): 8192 x 4096 x 8256 bf16 KK 414 .. 440 us = 1.26 .. 1.34 PFLOP/s (a 16 KiB row stride, K = 8192,
+// costs 15 %: the rows of a tile fall on the same channels), 16384 x 2048 x 8192 KM 429 .. 450 us = 1.22 .. 1.28 (490 in a pass, behind the launch that wrote dz),
+// 8192 x 2048 x 8192 MM 206 .. 216 us = 1.27 .. 1.34; fp32 4096^3 KM 0.99 ms = 0.139.  Bound by the issue of the LDS copies next to the matrix instructions
+// (SQ_VALU_MFMA_BUSY 57 % of the cycles); with all rows on one cache line the same loop reaches 1.38.
 // 64-byte steps in three to five buffers, or two groups of waves half a period apart, measured 0 .. 15 % slower.
 #include <algorithm>
 
@@ -394,8 +395,10 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g, long long pieces,
     epilogue8<T>(g.e, z, bias, m, n, g.N);
 }
 
-// ---- few rows (measured: 1 x 512 -> 256 fp32 in one launch of 3 us; W's read bounds wide layers, latency small ones): M <= 16 MB.  A work-group owns 16 columns; its waves split k and join through LDS.  W is read once, straight into fragments;
-// any K and any alignment. ----
+// ---- few rows: M <= 16 MB.  A work-group owns 16 columns; its waves split k and join through LDS.  W is read once, straight into fragments; any K and any
+// alignment.  Small layers are bound by latency (1 x 512 -> 256 fp32: one launch of 3 us), one row of a wide one by W's read (bf16, W out of HBM: 1 x 8192 ->
+// 8192 31.7 us = 4.2 TB/s, -> 32000 102 us = 5.1; fp32 60.5 us = 4.4 and 210 us = 5.0).  More rows are bound by reading x again in every work-group: 8192 -> 8192
+// bf16 41 us with 16 rows, 83 with 64 (fp32 79 and 188). ----
 template <class T>
 __device__ __forceinline__ typename Mma<T>::frag row_frag(const T* p, int k, int K) {
     typename Mma<T>::frag f;

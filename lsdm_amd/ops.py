@@ -6,20 +6,24 @@
                                                     backward passes read in that form
 
 They run in ``liblsdm_hip.so`` (include/lsdm_hip.h: ``lsdm_linear*``, ``lsdm_layer_norm*``, ``lsdm_pack8``, ``lsdm_unpack8``) on the current stream of
-the tensors' device (argument checks, allocation and autograd nodes: csrc/torch_ops.cpp); host tensors raise ``LsdmError``.  ``lsdm_amd.text.use_kernels`` puts them under a CLIP / BERT tower.
+the tensors' device (argument checks, allocation and autograd nodes: csrc/torch_ops.cpp); host tensors raise ``LsdmError``.
+``lsdm_amd.text.use_kernels`` puts them under a CLIP / BERT tower.
 
 Types: float32, bfloat16, float16, the same for all tensors of a call (``bias`` and the norm's ``weight`` / ``bias`` may also be float32).  Products
 accumulate and everything else is evaluated in 32 bits; results are rounded once.  In 16 bits the backward pass of ``linear`` rounds dz = dy a'(z) to the
 tensors' type, as the matrix cores take their operands in it (a'(z) itself is kept in 16 bits that round it by 2^-14 of its value near 1,
 2^-13 at 1/16 and 2^-8 at 1e-7).
-Shapes: any leading axes, any sizes including 0 rows (at most 2^30 rows and columns, 2^25 rows of ``weight``, 2^35 values of a checkpoint); the last axis should be contiguous (other layouts are copied first).
-Gradients are differentiable once; forward-mode derivatives there are none (a dual tensor raises ``LsdmError``).  Results do not depend on timing (no atomics): the same call gives the same bits.
+Shapes: any leading axes, any sizes including 0 rows (at most 2^30 rows and columns, 2^25 rows of ``weight``, 2^35 values of a checkpoint); the last axis
+should be contiguous (other layouts are copied first).
+Gradients are differentiable once; forward-mode derivatives there are none (a dual tensor raises ``LsdmError``).  Results do not depend on timing (no
+atomics): the same call gives the same bits.
 
 8-bit checkpoints: groups of 32 consecutive values of a row share a power-of-two step 2^e (e = max(floor(log2 max|x|) - 6, -126)); a value is kept
-as the int8 nearest to x / 2^e.  What is restored is exact in every type; a group that holds an infinity or a NaN comes back as NaN, so an overflow
-is never hidden.  ``linear(..., checkpoint8=True)`` keeps ``x`` in this form and a'(z) as one byte (step 1/192, exact at 0 and 1);
-``layer_norm(..., checkpoint8=True)`` keeps the normalised rows.  Codes taken from computed values flip on their last bit, which float32 gradients
-would show: in float32 ``linear`` keeps a'(z) in 32 bits, and ``layer_norm`` refuses ``checkpoint8``.
+as the int8 nearest to x / 2^e.  What is restored is exact in x's own type, bfloat16 and float32 (in float16 values of another type may lie outside its
+range); a group that holds an infinity or a NaN comes back as NaN, so an overflow is never hidden.  ``linear(..., checkpoint8=True)`` keeps ``x`` in this
+form and a'(z) as one byte (step 1/192, exact at 0 and 1); ``layer_norm(..., checkpoint8=True)`` keeps the normalised rows.  This is what is held between
+the passes: ``linear``'s backward pass restores one layer's ``x`` in full width as scratch memory while it runs.  Codes taken from computed values flip on
+their last bit, which float32 gradients would show: in float32 ``linear`` keeps a'(z) in 32 bits, and ``layer_norm`` refuses ``checkpoint8``.
 
 Tracers (``torch.jit.trace``, ``make_fx``, fake tensors) do not see what the kernels write: such calls raise ``LsdmError``.
 HIP graphs: forward and backward passes can be captured.  A leaf whose gradient node is held by a live autograd graph built eagerly on the default

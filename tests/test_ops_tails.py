@@ -175,3 +175,17 @@ def test_layer_norm_of_very_small_rows_without_eps(D, dt):
     # eps far above such rows' variance: h is next to nothing
     y = ops.layer_norm(x[[1, 3, 5]], eps=1e-5)
     base.norm_check(x[[1, 3, 5]], None, None, None, 1e-5, y, None)
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit checkpoints read back in other types
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+def test_checkpoints_are_exact_in_their_own_type_and_the_wide_ones(dt):
+    lo, hi = (-24, 14) if dt == "f16" else (-130, 126)
+    x = rows_of_scales(70, dt, range(lo, hi, 3), 7)
+    x = torch.where(x.isfinite(), x, torch.ones_like(x))
+    c = ops.checkpoint8(x)
+    want = base.stored8(x.double())
+    for t in {DT[dt], torch.float32, torch.bfloat16}:
+        assert torch.equal(c.restore(t).double(), want)
+    assert torch.equal(c.restore(torch.float16), want.half())                # elsewhere: the value in that type (an infinity beyond its range)
