@@ -12,6 +12,8 @@ of ``nn.Linear`` and ``nn.LayerNorm`` -- in place: parameters, names and ``state
 ``dense -> activation`` and ``dense -> + input -> LayerNorm``, its pooler, and CLIP's ``x + c_proj(gelu(c_fc(ln_2(x))))``; everything else is replaced
 layer by layer, and attention itself stays with the package.  A block whose layers carry hooks or were exchanged since runs its own ``forward``.
 Autocast does not reach the operators: give the tower the type instead (a call that mixes types raises ``ValueError``).
+bfloat16 towers and short prompt lists gain (BERT of 12 layers: 0.4 to 0.7 of the eager time); a float32 tower over 64 prompts and more takes 4 to 16 %
+longer than eager.
 """
 import functools
 import inspect
